@@ -272,6 +272,89 @@ qkv_status qkv_idx_read(qkv_engine *eng, int32_t layer, int32_t slot, int32_t po
 qkv_status qkv_attn_prefill(qkv_engine *eng, int32_t layer, int32_t slot, int32_t pos0,
                             const uint16_t *Q, int32_t Tc, float scale, float *out, void *stream);
 
+/* ------------------------------------------------------------------ ragged batches -------- */
+
+/* Maps of a ragged batch, built on the device from the sequences' lengths: n_new[i] >= 0 new rows
+ * of slots[i] (each slot at most once) at positions pos0[i] .. pos0[i]+n_new[i]-1, concatenated in
+ * order.  slots, pos0, n_new: HOST arrays [n_seq].  The rows' positions are reserved as qkv_append
+ * reserves them (pages allocated, shared pages copied, all or nothing over the batch; pos0[i] <=
+ * n_past) and n_past becomes max(n_past, pos0[i]+n_new[i]): the batch's rows are then to be appended
+ * in every layer (qkv_append_mapped).  Outputs, all device, all but cu_out nullable:
+ *   cu_out    [n_seq+1]   row offsets: sequence i holds rows cu[i] .. cu[i+1]-1
+ *   seq_out   [n_rows]    the row's sequence (index into slots)
+ *   pos_out   [n_rows]    the row's position
+ *   cell_out  [n_rows]    its cell in every layer's pool: page id * 256 + position % 256
+ *   table_out [n_seq][max_pages_per_seq]  page ids of positions 0 .. pos0+n_new-1, -1 behind them:
+ *             a qkv_cache_view.block_table of n_seq rows (qkv_attn_decode_static)
+ * n_rows >= the sum of n_new is the outputs' capacity: rows behind the last sequence get -1, so a
+ * captured graph can run a fixed number of rows over maps that are rebuilt before each replay.  The
+ * maps hold until one of the slots is reset, freed, restored or shared by a snapshot.  The reference
+ * holds one sequence whose cells are its positions (src/qwfn_state.h:14-16). */
+qkv_status qkv_batch_map(qkv_engine *eng, const int32_t *slots, const int32_t *pos0, const int32_t *n_new,
+                         int32_t n_seq, int32_t n_rows, int32_t *cu_out, int32_t *seq_out, int32_t *pos_out,
+                         int64_t *cell_out, int32_t *table_out, void *stream);
+/* Kernel A through a slot map: quantise row r of K and V (device F32 [n_rows][n_head_kv*head_dim],
+ * 16-byte aligned) to q8_0 as qkv_append does and store it in cell[r] (device, from qkv_batch_map) of
+ * layer `layer`; rows with cell -1 are skipped (and not read).  One launch for the rows of any number
+ * of sequences.  Host state is not touched (qkv_batch_map reserved the cells), so the call can be
+ * captured.  A cell outside the pool is skipped and sets the bad-index bit of qkv_device_status; two
+ * rows with the same cell leave one of them, or a mixture. */
+qkv_status qkv_append_mapped(qkv_engine *eng, int32_t layer, const int64_t *cell, const float *K, const float *V,
+                             int32_t n_rows, void *stream);
+
+/* ------------------------------------------------------------------ recurrent layers ------ */
+
+/* The kernels that advance the recurrent and convolution state of qkv_state_ptr in place, for
+ * engines with rec_head_dim 128, conv_hist 3 and conv_channels a multiple of 128 (else
+ * QKV_ERR_UNSUPPORTED).  slots: HOST array, each slot at most once; a slot's state starts as
+ * qkv_seq_reset, qkv_snapshot_restore or the caller left it (qkv_seq_alloc does not clear it).  With
+ * `save`, rollback snapshot s-1 of a slot receives the state s tokens back, s = 1 .. min(n_rollback, the
+ * slot's rows in this call); once every recurrent layer has run, declare them with qkv_rollback_arm.
+ * All calls can be captured: they upload nothing and use no workspace. */
+
+typedef enum qkv_dtype { QKV_F32 = 0, QKV_BF16 = 1 } qkv_dtype;
+
+/* Short causal convolution, silu and head norm over ragged rows (the reference's ggml_ssm_conv + silu +
+ * ggml_l2_norm in front of its DeltaNet, src/qwfn_graph.cpp:134-238):
+ *   y[t][c] = silu(sum_{j=0..3} w[c][j] * x[t-3+j][c]),
+ * the rows before a sequence's first being its history (state kind 1: [channel][3], oldest first),
+ * which then holds its last three rows; of the first n_norm channels (a multiple of 128: the heads of q
+ * and k) every 128 are divided by max(their 2-norm, eps).  cu: device int32 [n_seq+1] row offsets
+ * (qkv_batch_map); rows outside the sequences are neither read nor written, a sequence without rows
+ * keeps its state.  x: device rows of conv_channels values of `dtype`, x_stride elements apart; y:
+ * device [n_rows][conv_channels] of the same type, not overlapping x; w: device F32
+ * [conv_channels][4].  Pointers 16-byte aligned, x_stride a multiple of 16 bytes. */
+qkv_status qkv_rec_conv(qkv_engine *eng, int32_t rec_layer, const int32_t *slots, const int32_t *cu, int32_t n_seq,
+                        int32_t dtype, const void *x, int64_t x_stride, const float *w, int32_t n_rows,
+                        int32_t n_norm, float eps, void *y, int32_t save, void *stream);
+
+/* Rows of linear attention: value head h of rec_n_head reads head h / (rec_n_head / n_head_k) of q and
+ * k.  Row r's q and k are n_head_k heads of 128 at q + r * q_stride (elements), its v rec_n_head heads
+ * of 128 at v + r * v_stride; slices of one fused row are allowed.  g: F32 [rows][rec_n_head], the log
+ * of each head's decay (-inf allowed: the state is forgotten; +inf and NaN are not); beta: F32
+ * [rows][rec_n_head] for the gated delta rule, NULL for decay alone.  All device; q, k, v 16-byte
+ * aligned with strides of whole 16 bytes. */
+typedef struct qkv_rec_rows {
+    const void  *q, *k, *v;
+    int64_t      q_stride, k_stride, v_stride;
+    const float *g, *beta;
+    int32_t      n_head_k;
+} qkv_rec_rows;
+
+/* Recurrent form, T (1..4) tokens of n_seq sequences (rows i*T .. i*T+T-1 of sequence i).  Per value head
+ * with state S (kind 0: [head][value][key], key fastest), token by token:
+ *   S = e^g S;  u = beta * (v - S k), or u = v without beta;  S = S + u k^T;  out = scale * S q.
+ * q, k, v: F32 rows; out: F32 [n_seq*T][rec_n_head][128].  Replaces ggml_gated_delta_net of
+ * graph_builder::deltanet (src/qwfn_graph.cpp:210-238) and its rollback slots. */
+qkv_status qkv_rec_step(qkv_engine *eng, int32_t rec_layer, const int32_t *slots, int32_t n_seq,
+                        const qkv_rec_rows *rows, int32_t T, float scale, float *out, int32_t save, void *stream);
+/* Chunked form for prompts: the same recurrence over ragged rows, cu as in qkv_rec_conv; q, k, v: bf16
+ * rows; out: bf16 [n_rows][rec_n_head][128].  State, sums and decays are F32; out is rounded once
+ * at the end.  A row offset outside 0 .. n_rows, or a falling one, skips that sequence and sets the
+ * bad-index bit of qkv_device_status. */
+qkv_status qkv_rec_chunk(qkv_engine *eng, int32_t rec_layer, const int32_t *slots, const int32_t *cu, int32_t n_seq,
+                         const qkv_rec_rows *rows, int32_t n_rows, float scale, uint16_t *out, void *stream);
+
 /* ------------------------------------------------------------------ kernel E -------------- */
 
 /* Snapshot of a slot's first n_past positions: its pages are shared (refcounted, no KV bytes

@@ -10,6 +10,7 @@ missing or fails to load, importing the engine raises.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 from dataclasses import dataclass, field
 
@@ -31,8 +32,11 @@ EXPORTS = [
     "qkv_store_prefix_split", "qkv_store_evict", "qkv_store_info", "qkv_store_entry",
     "qkv_indexer_enable", "qkv_idx_append", "qkv_idx_select", "qkv_attn_decode_qsa", "qkv_idx_read",
     "qkv_project_append", "qkv_static_status", "qkv_debug_decode_wait", "qkv_attn_prefill_qsa",
-    "qkv_debug_check_q8_scale",
+    "qkv_debug_check_q8_scale", "qkv_batch_map", "qkv_append_mapped", "qkv_rec_conv", "qkv_rec_step",
+    "qkv_rec_chunk",
 ]
+
+F32, BF16 = range(2)   # qkv_dtype
 
 
 class QkvError(RuntimeError):
@@ -59,6 +63,12 @@ class QkvCacheView(ctypes.Structure):
                 ("page_tokens", ctypes.c_int32), ("tile_tokens", ctypes.c_int32), ("n_pages", ctypes.c_int32),
                 ("n_head_kv", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("block_table", ctypes.c_void_p),
                 ("max_pages_per_seq", ctypes.c_int32)]
+
+
+class QkvRecRows(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_stride", ctypes.c_int64),
+                ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64), ("g", ctypes.c_void_p),
+                ("beta", ctypes.c_void_p), ("n_head_k", ctypes.c_int32)]
 
 
 _lib = None
@@ -119,6 +129,11 @@ def lib() -> ctypes.CDLL:
         "qkv_static_status": [P, pI32],
         "qkv_debug_decode_wait": [P, I64, I32],
         "qkv_attn_prefill_qsa": [P, I32, I32, I32, P, P, I32, F32, P, P, P, P],
+        "qkv_batch_map": [P, pI32, pI32, pI32, I32, I32, P, P, P, P, P, P],
+        "qkv_append_mapped": [P, I32, P, P, P, I32, P],
+        "qkv_rec_conv": [P, I32, pI32, P, I32, I32, P, I64, P, I32, I32, F32, P, I32, P],
+        "qkv_rec_step": [P, I32, pI32, I32, ctypes.POINTER(QkvRecRows), I32, F32, P, I32, P],
+        "qkv_rec_chunk": [P, I32, pI32, P, I32, ctypes.POINTER(QkvRecRows), I32, F32, P, P],
         "qkv_debug_check_q8_scale": [ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64)],
     }
     for name, args in sig.items():
@@ -147,6 +162,27 @@ def _ptr(x) -> int | None:
         return x
     if not x.is_contiguous():
         raise ValueError("tensor must be contiguous")
+    return x.data_ptr()
+
+
+def _rows(x, dtype: str):
+    """Pointer and row stride (elements) of a tensor of rows [n, ...] whose rows are contiguous."""
+    if str(x.dtype) != dtype:
+        raise ValueError(f"rows of {dtype} wanted, got {x.dtype}")
+    want = 1
+    for d in range(x.dim() - 1, 0, -1):
+        if x.shape[d] > 1 and x.stride(d) != want:
+            raise ValueError("each row must be contiguous")
+        want *= x.shape[d]
+    return x.data_ptr(), x.stride(0) if x.shape[0] > 1 else max(x.stride(0), want)
+
+
+def _dense(x, dtype: str, n: int, what: str):
+    """Pointer of a contiguous tensor of dtype with at least n elements; None -> NULL."""
+    if x is None:
+        return None
+    if str(x.dtype) != dtype or not x.is_contiguous() or x.numel() < n:
+        raise ValueError(f"{what}: contiguous {dtype} of at least {n} elements wanted, got {x.dtype} {tuple(x.shape)}")
     return x.data_ptr()
 
 
@@ -422,6 +458,91 @@ class Engine:
         self._check(lib().qkv_project_append(self.handle, layer, slot, pos, _ptr(x), n_embd, T, _ptr(Wq), _ptr(Wk),
                                              _ptr(Wv), _ptr(q_norm), _ptr(k_norm), rms_eps, rope_dim, rope_freq_base,
                                              _ptr(Q_out), _stream(stream)))
+
+    # -- ragged batches ------------------------------------------------------------------------
+    def batch_map(self, slots, pos0, n_new, n_rows: int, cu, seq=None, pos=None, cell=None, table=None,
+                  stream=None) -> None:
+        """Row offsets, sequences, positions, cells and block tables of a ragged batch (include/qkv.h
+        qkv_batch_map); int32 device tensors, cell int64."""
+        n = len(slots)
+        if len(pos0) != n or len(n_new) != n:
+            raise ValueError(f"{n} slots, {len(pos0)} positions, {len(n_new)} lengths")
+        ctx = self.cfg.n_ctx
+        self._check(lib().qkv_batch_map(
+            self.handle, _i32_array(slots), _i32_array(pos0), _i32_array(n_new), n, n_rows,
+            _dense(cu, "torch.int32", n + 1, "cu"), _dense(seq, "torch.int32", n_rows, "seq"),
+            _dense(pos, "torch.int32", n_rows, "pos"), _dense(cell, "torch.int64", n_rows, "cell"),
+            _dense(table, "torch.int32", n * ((ctx + 255) // 256), "table"), _stream(stream) if self.device >= 0 else None))
+
+    def append_mapped(self, layer: int, cell, K, V, stream=None) -> None:
+        """Quantise F32 rows [n, n_head_kv * head_dim] into the cells of a slot map; -1 skips a row."""
+        n = int(K.shape[0])
+        w = n * self.cfg.n_head_kv * self.cfg.head_dim
+        self._check(lib().qkv_append_mapped(self.handle, layer, _dense(cell, "torch.int64", n, "cell"),
+                                            _dense(K, "torch.float32", w, "K"), _dense(V, "torch.float32", w, "V"), n,
+                                            _stream(stream)))
+
+    # -- recurrent layers ----------------------------------------------------------------------
+    def rec_state(self, rec_layer: int, kind: int = 0, which: int = 0):
+        """torch view of every slot's recurrent state (kind 0: [n_slots, head, value, key]) or convolution
+        history (kind 1: [n_slots, channel, 3]) in place; which > 0: rollback snapshot which - 1."""
+        import torch
+        c = self.cfg
+        base, _ = self.state_ptr(0, rec_layer, kind, which)
+        step = self.state_ptr(1, rec_layer, kind, which)[0] - base if c.n_slots > 1 else 0
+        shape = (c.rec_n_head, c.rec_head_dim, c.rec_head_dim) if kind == 0 else (c.conv_channels, c.conv_hist)
+        strides, at = [], 4
+        for s in reversed(shape):
+            strides.insert(0, at)
+            at *= s
+        view = type("RecState", (), {})()
+        view.__cuda_array_interface__ = {"shape": (c.n_slots, *shape), "strides": (step or at, *strides), "typestr": "<f4",
+                                         "data": (base, False), "version": 3}
+        view.engine = self   # the memory is the engine's: keep it while the view lives
+        return torch.as_tensor(view, device=f"cuda:{self.device}")
+
+    def rec_conv(self, rec_layer: int, slots, cu, x, w, y, n_norm: int = 0, eps: float = 1e-6, save: bool = False,
+                 stream=None) -> None:
+        """Causal convolution of width 4 + silu over ragged rows, heads of the first n_norm channels normalised.
+        x: F32 or bf16 rows [n, conv_channels] (a stride between rows is allowed); y: same type, contiguous."""
+        kind = str(x.dtype)
+        if kind not in ("torch.float32", "torch.bfloat16") or x.dim() != 2 or x.shape[1] != self.cfg.conv_channels:
+            raise ValueError(f"x: F32 or bf16 [n, {self.cfg.conv_channels}] wanted, got {x.dtype} {tuple(x.shape)}")
+        n = int(x.shape[0])
+        ptr, stride = _rows(x, kind)
+        self._check(lib().qkv_rec_conv(
+            self.handle, rec_layer, _i32_array(slots), _dense(cu, "torch.int32", len(slots) + 1, "cu"), len(slots),
+            F32 if kind == "torch.float32" else BF16, ptr, stride,
+            _dense(w, "torch.float32", 4 * self.cfg.conv_channels, "w"), n, n_norm, eps,
+            _dense(y, kind, n * self.cfg.conv_channels, "y"), int(save), _stream(stream)))
+
+    def _rec_rows(self, q, k, v, g, beta, n: int, dtype: str) -> QkvRecRows:
+        H, hd = self.cfg.rec_n_head, self.cfg.rec_head_dim
+        width, wk, wv = (math.prod(t.shape[1:]) for t in (q, k, v))
+        if any(int(t.shape[0]) != n for t in (q, k, v)) or width % hd or wk != width or wv != H * hd:
+            raise ValueError(f"{n} rows of q and k [heads * {hd}] and v [{H} * {hd}] wanted: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+        (qp, qs), (kp, ks), (vp, vs) = (_rows(t, dtype) for t in (q, k, v))
+        return QkvRecRows(qp, kp, vp, qs, ks, vs, _dense(g, "torch.float32", n * H, "g"),
+                          _dense(beta, "torch.float32", n * H, "beta"), width // hd)
+
+    def rec_step(self, rec_layer: int, slots, q, k, v, g, beta, T: int, scale: float, out, save: bool = False,
+                 stream=None) -> None:
+        """Linear attention with a decay per head (beta: the gated delta rule; None: decay alone), T (1..4) F32
+        rows per sequence; the state advances in place."""
+        n = len(slots) * T
+        rows = self._rec_rows(q, k, v, g, beta, n, "torch.float32")
+        self._check(lib().qkv_rec_step(self.handle, rec_layer, _i32_array(slots), len(slots), ctypes.byref(rows), T, scale,
+                                       _dense(out, "torch.float32", n * self.cfg.rec_n_head * self.cfg.rec_head_dim, "out"),
+                                       int(save), _stream(stream)))
+
+    def rec_chunk(self, rec_layer: int, slots, cu, q, k, v, g, beta, scale: float, out, stream=None) -> None:
+        """The same recurrence over the ragged bf16 rows of prompts (cu: row offsets), in chunks."""
+        n = int(q.shape[0])
+        rows = self._rec_rows(q, k, v, g, beta, n, "torch.bfloat16")
+        self._check(lib().qkv_rec_chunk(self.handle, rec_layer, _i32_array(slots),
+                                        _dense(cu, "torch.int32", len(slots) + 1, "cu"), len(slots), ctypes.byref(rows), n, scale,
+                                        _dense(out, "torch.bfloat16", n * self.cfg.rec_n_head * self.cfg.rec_head_dim, "out"),
+                                        _stream(stream)))
 
     # -- QSA lightning indexer ------------------------------------------------------------------
     def indexer_enable(self, n_head: int = 4, top_k: int = 2048, rope_dim: int = 64, rope_freq_base: float = 1e7,

@@ -1384,6 +1384,212 @@ extern "C" qkv_status qkv_attn_prefill_qsa(qkv_engine *eng, int32_t layer, int32
     return prefill_run(eng, layer, slot, pos0, Q, Tc, scale, out, eng->d_pbits, words, stream);
 }
 
+// --------------------------------------------------------------------------- ragged batches
+// Slots valid and each named once.
+static qkv_status check_slots(qkv_engine *eng, const int32_t *slots, int32_t n_seq, const char *what) {
+    std::vector<uint8_t> seen(eng->cfg.n_slots, 0);
+    for (int32_t i = 0; i < n_seq; i++) {
+        const qkv_status r = check_slot(eng, slots[i]);
+        if (r != QKV_OK) return r;
+        if (seen[slots[i]]++) return fail(eng, QKV_ERR_INVALID, "%s: slot %d twice", what, slots[i]);
+    }
+    return QKV_OK;
+}
+static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+extern "C" qkv_status qkv_batch_map(qkv_engine *eng, const int32_t *slots, const int32_t *pos0, const int32_t *n_new,
+                                    int32_t n_seq, int32_t n_rows, int32_t *cu_out, int32_t *seq_out, int32_t *pos_out,
+                                    int64_t *cell_out, int32_t *table_out, void *stream) {
+    if (!eng) return QKV_ERR_INVALID;
+    qkv_status r;
+    if (!slots || !pos0 || !n_new || n_seq < 1 || n_rows < 0 || !cu_out)
+        return fail(eng, QKV_ERR_INVALID, "batch_map: n_seq %d, n_rows %d, null pointer", n_seq, n_rows);
+    if ((r = check_slots(eng, slots, n_seq, "batch_map")) != QKV_OK) return r;
+    int64_t total = 0;
+    size_t need = 0;
+    for (int32_t i = 0; i < n_seq; i++) {
+        const qkv_engine::Slot &sl = eng->slots[slots[i]];
+        if (n_new[i] < 0 || pos0[i] < 0 || pos0[i] > sl.n_past)
+            return fail(eng, QKV_ERR_INVALID, "batch_map: %d rows at %d: slot %d holds %d positions", n_new[i], pos0[i], slots[i], sl.n_past);
+        if ((int64_t)pos0[i] + n_new[i] > eng->cfg.n_ctx)
+            return fail(eng, QKV_ERR_STATE, "context exhausted: %d + %d > n_ctx %d", pos0[i], n_new[i], eng->cfg.n_ctx);
+        total += n_new[i];
+        for (int32_t pi = pos0[i] / PAGE_TOK; n_new[i] > 0 && pi <= (pos0[i] + n_new[i] - 1) / PAGE_TOK; pi++)
+            if (pi >= (int32_t)sl.pages.size() || eng->refcnt[sl.pages[pi]] > 1) need++;
+    }
+    if (total > n_rows) return fail(eng, QKV_ERR_INVALID, "batch_map: %lld new rows, outputs hold %d", (long long)total, n_rows);
+    if (need > eng->free_pages.size())
+        return fail(eng, QKV_ERR_NO_MEMORY, "page pool exhausted: need %zu pages, %zu free", need, eng->free_pages.size());
+    if (!eng->host_only && (r = use_device(eng)) != QKV_OK) return r;
+    cudaStream_t st = S(stream);
+    for (int32_t i = 0; i < n_seq; i++) {
+        if (n_new[i] == 0) continue;
+        if ((r = reserve(eng, slots[i], pos0[i], n_new[i], st)) != QKV_OK) return r;
+        qkv_engine::Slot &sl = eng->slots[slots[i]];
+        sl.n_past = std::max(sl.n_past, pos0[i] + n_new[i]);
+        invalidate_summaries(eng, slots[i], pos0[i]);
+    }
+    if (eng->host_only) return fail(eng, QKV_ERR_UNSUPPORTED, "host-only engine: pages reserved, no maps written");
+    if ((r = flush_tables(eng, st)) != QKV_OK) return r;
+    int32_t row = 0;
+    for (int32_t base = 0; base < n_seq; base += BM_SEQ) {
+        BatchMapParams p;
+        memset(&p, 0, sizeof p);
+        p.bt = eng->d_bt;
+        p.cu_out = cu_out;
+        p.seq_out = seq_out;
+        p.pos_out = pos_out;
+        p.cell_out = cell_out;
+        p.table_out = table_out;
+        p.status = eng->d_status;
+        p.n_seq = std::min(BM_SEQ, n_seq - base);
+        p.seq0 = base;
+        p.max_pages = eng->max_pages;
+        p.n_pages = eng->n_pages;
+        p.row_lo = row;
+        for (int32_t i = 0; i < p.n_seq; i++) {
+            p.slot[i] = slots[base + i];
+            p.pos0[i] = pos0[base + i];
+            p.cu[i] = row;
+            row += n_new[base + i];
+        }
+        p.cu[p.n_seq] = row;
+        p.row_hi = base + p.n_seq == n_seq ? n_rows : row;
+        CK(eng, launch_batch_map(p, st));
+    }
+    return QKV_OK;
+}
+
+extern "C" qkv_status qkv_append_mapped(qkv_engine *eng, int32_t layer, const int64_t *cell, const float *K, const float *V,
+                                        int32_t n_rows, void *stream) {
+    if (!eng) return QKV_ERR_INVALID;
+    qkv_status r;
+    if ((r = check_layer(eng, layer)) != QKV_OK) return r;
+    if (n_rows < 1 || !cell || !K || !V || !aligned16(K) || !aligned16(V))
+        return fail(eng, QKV_ERR_INVALID, "append_mapped: %d rows, null or unaligned pointer", n_rows);
+    if ((r = use_device(eng)) != QKV_OK) return r;
+    CK(eng, launch_append_mapped(pool_ref(eng, layer, eng->d_bt), cell, K, V, n_rows, S(stream)));
+    return QKV_OK;
+}
+
+// ------------------------------------------------------------------------- recurrent layers
+static qkv_status rec_check(qkv_engine *eng, int32_t rec_layer, const int32_t *slots, int32_t n_seq, int32_t save, const char *what) {
+    if (rec_layer < 0 || rec_layer >= eng->cfg.rec_n_layer)
+        return fail(eng, QKV_ERR_INVALID, "%s: recurrent layer %d outside [0, %d)", what, rec_layer, eng->cfg.rec_n_layer);
+    if (!slots || n_seq < 1) return fail(eng, QKV_ERR_INVALID, "%s: n_seq %d, null pointer", what, n_seq);
+    if (save && eng->cfg.n_rollback < 1) return fail(eng, QKV_ERR_INVALID, "%s: save on an engine without rollback snapshots", what);
+    return check_slots(eng, slots, n_seq, what);
+}
+
+extern "C" qkv_status qkv_rec_conv(qkv_engine *eng, int32_t rec_layer, const int32_t *slots, const int32_t *cu, int32_t n_seq,
+                                   int32_t dtype, const void *x, int64_t x_stride, const float *w, int32_t n_rows,
+                                   int32_t n_norm, float eps, void *y, int32_t save, void *stream) {
+    if (!eng) return QKV_ERR_INVALID;
+    qkv_status r;
+    if ((r = rec_check(eng, rec_layer, slots, n_seq, save, "rec_conv")) != QKV_OK) return r;
+    const qkv_config &c = eng->cfg;
+    if (c.conv_hist != 3 || c.conv_channels % 128)
+        return fail(eng, QKV_ERR_UNSUPPORTED, "rec_conv: conv_hist %d (3), conv_channels %d (a multiple of 128)", c.conv_hist, c.conv_channels);
+    const int64_t esz = dtype == QKV_F32 ? 4 : 2;
+    if ((dtype != QKV_F32 && dtype != QKV_BF16) || !cu || !x || !w || !y || n_rows < 1 || n_norm < 0 || n_norm % 128 ||
+        n_norm > c.conv_channels || !(eps >= 0.f) || !aligned16(x) || !aligned16(w) || !aligned16(y) ||
+        x_stride < c.conv_channels || x_stride * esz % 16)
+        return fail(eng, QKV_ERR_INVALID, "rec_conv: dtype %d, %d rows %lld apart, n_norm %d, null or unaligned pointer", dtype, n_rows,
+                    (long long)x_stride, n_norm);
+    const uint8_t *x0 = (const uint8_t *)x, *y0 = (const uint8_t *)y;
+    if (x0 < y0 + (int64_t)n_rows * c.conv_channels * esz && y0 < x0 + ((int64_t)(n_rows - 1) * x_stride + c.conv_channels) * esz)
+        return fail(eng, QKV_ERR_INVALID, "rec_conv: y overlaps x");
+    if ((r = use_device(eng)) != QKV_OK) return r;
+    for (int32_t base = 0; base < n_seq; base += MAX_SEQ) {
+        RecConvParams p;
+        memset(&p, 0, sizeof p);
+        p.x = x;
+        p.y = y;
+        p.w = w;
+        p.cu = cu + base;
+        const int64_t off = (int64_t)rec_layer * eng->rec_layer_bytes + eng->rs_bytes;
+        p.state = eng->d_rec + off;
+        p.back = eng->d_rb + off;
+        p.x_stride = x_stride;
+        p.slot_bytes = eng->rec_slot_bytes;
+        p.n_seq = std::min(MAX_SEQ, n_seq - base);
+        p.n_rows = n_rows;
+        p.channels = c.conv_channels;
+        p.n_norm = n_norm;
+        p.n_rollback = c.n_rollback;
+        p.n_save = save ? c.n_rollback : 0;
+        p.eps = eps;
+        std::copy(slots + base, slots + base + p.n_seq, p.slot);
+        CK(eng, launch_rec_conv(p, dtype == QKV_BF16, eng->num_sms, S(stream)));
+    }
+    return QKV_OK;
+}
+
+static qkv_status rec_attn(qkv_engine *eng, int32_t rec_layer, const int32_t *slots, const int32_t *cu, int32_t n_seq,
+                           const qkv_rec_rows *rows, int32_t n_rows, int32_t T, float scale, void *out, int32_t save,
+                           void *stream, const char *what) {
+    if (!eng) return QKV_ERR_INVALID;
+    qkv_status r;
+    if ((r = rec_check(eng, rec_layer, slots, n_seq, save, what)) != QKV_OK) return r;
+    const qkv_config &c = eng->cfg;
+    if (c.rec_head_dim != REC_HD) return fail(eng, QKV_ERR_UNSUPPORTED, "%s: rec_head_dim %d (128)", what, c.rec_head_dim);
+    const bool step = T > 0;
+    const int64_t per16 = step ? 4 : 8;
+    if (!rows || !out || !rows->q || !rows->k || !rows->v || !rows->g || rows->n_head_k < 1 || c.rec_n_head % rows->n_head_k ||
+        !aligned16(rows->q) || !aligned16(rows->k) || !aligned16(rows->v) || !aligned16(out) ||
+        rows->q_stride < (int64_t)rows->n_head_k * REC_HD || rows->k_stride < (int64_t)rows->n_head_k * REC_HD ||
+        rows->v_stride < (int64_t)c.rec_n_head * REC_HD || rows->q_stride % per16 || rows->k_stride % per16 || rows->v_stride % per16)
+        return fail(eng, QKV_ERR_INVALID, "%s: n_head_k %d of %d heads, null or unaligned pointer, stride below a row or not a multiple of 16 bytes",
+                    what, rows ? rows->n_head_k : 0, c.rec_n_head);
+    if ((r = use_device(eng)) != QKV_OK) return r;
+    const int64_t esz = step ? 4 : 2;
+    for (int32_t base = 0; base < n_seq; base += MAX_SEQ) {
+        RecParams p;
+        memset(&p, 0, sizeof p);
+        const int64_t r0 = step ? (int64_t)base * T : 0;   // the step's rows of this launch
+        p.q = (const uint8_t *)rows->q + r0 * rows->q_stride * esz;
+        p.k = (const uint8_t *)rows->k + r0 * rows->k_stride * esz;
+        p.v = (const uint8_t *)rows->v + r0 * rows->v_stride * esz;
+        p.g = rows->g + r0 * c.rec_n_head;
+        p.beta = rows->beta ? rows->beta + r0 * c.rec_n_head : nullptr;
+        p.out = (uint8_t *)out + r0 * c.rec_n_head * REC_HD * esz;
+        p.cu = cu ? cu + base : nullptr;
+        const int64_t off = (int64_t)rec_layer * eng->rec_layer_bytes;
+        p.state = eng->d_rec + off;
+        p.back = eng->d_rb + off;
+        p.status = eng->d_status;
+        p.q_stride = rows->q_stride;
+        p.k_stride = rows->k_stride;
+        p.v_stride = rows->v_stride;
+        p.slot_bytes = eng->rec_slot_bytes;
+        p.n_seq = std::min(MAX_SEQ, n_seq - base);
+        p.n_rows = step ? p.n_seq * T : n_rows;
+        p.T = T;
+        p.n_head = c.rec_n_head;
+        p.n_head_k = rows->n_head_k;
+        p.n_rollback = c.n_rollback;
+        p.n_save = save ? c.n_rollback : 0;
+        p.scale = scale;
+        std::copy(slots + base, slots + base + p.n_seq, p.slot);
+        CK(eng, step ? launch_rec_step(p, S(stream)) : launch_rec_chunk(p, S(stream)));
+    }
+    return QKV_OK;
+}
+
+extern "C" qkv_status qkv_rec_step(qkv_engine *eng, int32_t rec_layer, const int32_t *slots, int32_t n_seq,
+                                   const qkv_rec_rows *rows, int32_t T, float scale, float *out, int32_t save, void *stream) {
+    if (!eng) return QKV_ERR_INVALID;
+    if (T < 1 || T > 4) return fail(eng, QKV_ERR_INVALID, "rec_step: T %d (1..4)", T);
+    return rec_attn(eng, rec_layer, slots, nullptr, n_seq, rows, 0, T, scale, out, save, stream, "rec_step");
+}
+
+extern "C" qkv_status qkv_rec_chunk(qkv_engine *eng, int32_t rec_layer, const int32_t *slots, const int32_t *cu, int32_t n_seq,
+                                    const qkv_rec_rows *rows, int32_t n_rows, float scale, uint16_t *out, void *stream) {
+    if (!eng) return QKV_ERR_INVALID;
+    if (!cu || n_rows < 1) return fail(eng, QKV_ERR_INVALID, "rec_chunk: %d rows, null pointer", n_rows);
+    return rec_attn(eng, rec_layer, slots, cu, n_seq, rows, n_rows, 0, scale, out, 0, stream, "rec_chunk");
+}
+
 // -------------------------------------------------------------------------------- snapshots
 static qkv_status rec_copy(qkv_engine *eng, const std::vector<CopyDesc> &d, cudaStream_t st) {
     if (d.empty() || eng->host_only) return QKV_OK;

@@ -298,6 +298,56 @@ struct alignas(16) PfPlanInline {
 cudaError_t launch_prefill(const PrefillParams &p, const PfPlanInline &plan, cudaStream_t st);
 int prefill_max_pairs();   // co-resident CTA pairs of kernel D (0 = unknown)
 
+// ---- ragged batches (qkv_batch.cu) ---------------------------------------------------------------
+constexpr int BM_SEQ = 256;               // sequences per map launch (their lengths are kernel parameters)
+struct BatchMapParams {
+    const int32_t *bt;                    // engine block table [n_slots][max_pages]
+    int32_t *cu_out;                      // [all sequences + 1]
+    int32_t *seq_out, *pos_out;           // nullable [rows]
+    int64_t *cell_out;                    // nullable [rows]
+    int32_t *table_out;                   // nullable [all sequences][max_pages]
+    int32_t *status;
+    int32_t n_seq, seq0;                  // this launch's sequences: seq0 .. seq0 + n_seq - 1
+    int32_t row_lo, row_hi;               // rows that this launch writes (rows of no sequence: -1)
+    int32_t max_pages, n_pages;
+    int32_t row_blocks;                   // set by launch_batch_map
+    int32_t slot[BM_SEQ], pos0[BM_SEQ], cu[BM_SEQ + 1];
+};
+cudaError_t launch_batch_map(BatchMapParams &p, cudaStream_t st);
+cudaError_t launch_append_mapped(const PoolRef &pr, const int64_t *cell, const float *K, const float *V, int32_t n_rows,
+                                 cudaStream_t st);
+
+// ---- recurrent layers (qkv_recurrent.cu) ---------------------------------------------------------
+constexpr int REC_HD = 128;               // head size of the recurrent layers' kernels
+struct RecConvParams {
+    const void    *x;                     // F32 or bf16 rows, x_stride apart
+    void          *y;                     // same type [n_rows][channels]
+    const float   *w;                     // [channels][4]
+    const int32_t *cu;                    // device [n_seq + 1]
+    uint8_t       *state, *back;          // the layer's history of slot 0 / of slot 0's rollback snapshot 0
+    int64_t x_stride, slot_bytes;
+    int32_t n_seq, n_rows, channels, n_norm, n_rollback, n_save;
+    float   eps;
+    int32_t rows_per;                     // set by launch_rec_conv
+    int32_t slot[MAX_SEQ];
+};
+cudaError_t launch_rec_conv(RecConvParams &p, bool bf16, int num_sms, cudaStream_t st);
+
+struct RecParams {
+    const void    *q, *k, *v;             // rows of n_head_k (q, k) or n_head (v) heads of REC_HD
+    const float   *g, *beta;              // [rows][n_head]; beta nullable (no delta rule)
+    void          *out;                   // [rows][n_head][REC_HD], the type of q, k, v
+    const int32_t *cu;                    // device [n_seq + 1], or null: T rows per sequence
+    uint8_t       *state, *back;          // the layer's state of slot 0 / of slot 0's rollback snapshot 0
+    int32_t       *status;
+    int64_t q_stride, k_stride, v_stride, slot_bytes;
+    int32_t n_seq, n_rows, T, n_head, n_head_k, n_rollback, n_save;
+    float   scale;
+    int32_t slot[MAX_SEQ];
+};
+cudaError_t launch_rec_step(const RecParams &p, cudaStream_t st);    // F32, a few tokens per sequence
+cudaError_t launch_rec_chunk(const RecParams &p, cudaStream_t st);   // bf16, ragged prompts
+
 // ---- host side shared by the engine and the saved-sequence store (qkv_store.cpp) ---------------
 // Sets the engine's last error (qkv_last_error) to msg and returns st.
 qkv_status engine_fail(qkv_engine *eng, qkv_status st, const char *msg);
