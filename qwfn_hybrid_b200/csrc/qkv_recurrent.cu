@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 namespace qkv {
 
@@ -320,6 +321,663 @@ __global__ void __launch_bounds__(RT_THREADS) k_rec_serial(const __grid_constant
     }
 }
 
+// ------------------------------------------------------------------------ chunked linear attention
+// 64 tokens at a time.  With G = sums of g inside the chunk (G_C: the whole chunk's) and S the state before it,
+//   A_ij = beta_i (k_i . k_j) e^(G_i - G_j) for j < i,   T = (1 + A)^-1   (lower triangular),
+//   U = T R,  R_j = beta_j (v_j - e^(G_j) S k_j)          (without the delta rule U = V),
+//   o_i = scale (e^(G_i) S q_i + sum_{j <= i} (q_i . k_j) e^(G_i - G_j) u_j),
+//   S  <- e^(G_C) S + sum_j e^(G_C - G_j) u_j k_j^T.
+// A CTA owns RK_NW * 16 value rows of one head of one sequence and walks its chunks; value rows need nothing
+// from one another, so heads and sequences fill the GPU.  Everything without S -- k and q as f16,
+// the scores P, T -- is made by RK_PROD producer threads one chunk ahead (two stages in shared memory); the chain
+// through S is carried by RK_NW warps of 16 value rows each, wholly in registers: with value rows as the M
+// of every product the accumulator of one product (rows: values, columns: tokens or keys) is, register for
+// register, the A operand of the next (S -> S k -> R -> U -> S), so the chain has no shared memory,
+// shuffle or barrier between its products.  The warps meet at named barriers (no spinning).
+// Why mma.sync and not tcgen05: the chain is serial, five dependent products of 16 x 64 x 128 or less per warp
+// and chunk; through tensor memory every one of them would add a commit, a wait and a round trip of
+// tcgen05.ld and a store, which cost more than these products.
+//
+// Precision.  bf16 inputs are exact in f16 once a power of two has brought the row's largest value to
+// [1, 2); S, R, T and U enter as two f16 terms of a row scaled to [2^12, 2^13) (hi + lo: 22 bits), three
+// products where both operands are split, so state and U keep 32-bit accuracy with 16-bit instructions.  The output
+// is rounded to bf16, so its two products take the leading term alone (11 bits against 8).  Sums are F32;
+// the state is scaled and added outside the tensor cores (their sums are truncated).  G is summed in
+// 64 bits and kept as two floats: e^(G_i - G_j) needs the difference, not the rounded sums.
+//
+// A zero of T or P times a NaN is a NaN, so a chunk with a non-finite input would spread it to earlier
+// tokens; such chunks are flagged by the producers and run token by token from global memory.
+constexpr int RK_C = 64, RK_NW = 4, RK_PROD = 256, RK_THREADS = RK_PROD + RK_NW * 32;
+constexpr int RK_ROWS = RK_NW * 16;
+constexpr int RK_K = 0, RK_Q = 16384, RK_P = 32768, RK_TH = 40960, RK_TL = 49152, RK_V = 57344;
+constexpr int RK_COEF = RK_V + RK_C * RK_ROWS * 2;      // six arrays of RK_C floats, then e^(G_C) and the flag
+enum { CF_X, CF_V, CF_T, CF_Q1, CF_Q2, CF_W, CF_N };
+constexpr int RK_STAGE = RK_COEF + CF_N * RK_C * 4 + 128;
+constexpr int RK_PITCH = 68;                            // floats per row of the producers' triangular matrices
+constexpr int RK_A = 2 * RK_STAGE, RK_T = RK_A + RK_C * RK_PITCH * 4, RK_SMALL = RK_T + RK_C * RK_PITCH * 4;
+constexpr int RK_SMEM = RK_SMALL + 6 * RK_C * 4;
+enum { BAR_FULL = 1, BAR_EMPTY = 3, BAR_PROD = 5 };
+
+__device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ void bar_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void stsm4t(uint32_t addr, const uint32_t (&r)[4]) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]) : "memory");
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The power of two that brings a row whose largest magnitude is m to [2^TE, 2^(TE+1)), and its inverse
+// (both normal numbers; rows below 2^(TE-126) are left smaller).
+template <int TE>
+__device__ __forceinline__ float pow2_scale(float m, float &inv) {
+    const int e = (__float_as_int(m) >> 23) & 255;
+    const int f = min(254 + TE - e, 253);
+    inv = __int_as_float((254 - f) << 23);
+    return __int_as_float(f << 23);
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ void split_f16(float a, float b, float s, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(a * s, b * s);
+    const float2 f = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = pack_f16(fmaf(a, s, -f.x), fmaf(b, s, -f.y));
+}
+__device__ __forceinline__ float quad_max(float v) {
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    v += __shfl_xor_sync(0xffffffffu, v, 1);
+    return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+// Row scales of an accumulator tile set (rows g and g + 8 of the lane's quad).
+template <int N>
+__device__ __forceinline__ void row_scales(const float (&x)[N][4], float &s0, float &s1, float &i0, float &i1) {
+    float m0 = 0.0f, m1 = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        m0 = fmaxf(m0, fmaxf(fabsf(x[n][0]), fabsf(x[n][1])));
+        m1 = fmaxf(m1, fmaxf(fabsf(x[n][2]), fabsf(x[n][3])));
+    }
+    s0 = pow2_scale<12>(quad_max(m0), i0);
+    s1 = pow2_scale<12>(quad_max(m1), i1);
+}
+
+// The chunk's inputs of a producer thread, loaded one chunk ahead: 4 x 16 bytes of k and of q (rows
+// 16 p + tid / 16, chunk tid % 16), 2 of v (rows 32 p + tid / 8, chunk tid % 8), g and beta of token tid.
+struct RkIn {
+    uint4 k[4], q[4], v[2];
+    float g, b;
+};
+__device__ __forceinline__ void rk_load(RkIn &in, const RecParams &p, const __nv_bfloat16 *k, const __nv_bfloat16 *q,
+                                        const __nv_bfloat16 *v, int h, int32_t t0, int32_t end, int tid) {
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int32_t r = t0 + 16 * i + (tid >> 4);
+        const bool ok = r < end;
+        in.k[i] = ok ? *reinterpret_cast<const uint4 *>(k + (int64_t)r * p.k_stride + (tid & 15) * 8) : zero;
+        in.q[i] = ok ? *reinterpret_cast<const uint4 *>(q + (int64_t)r * p.q_stride + (tid & 15) * 8) : zero;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int32_t r = t0 + 32 * i + (tid >> 3);
+        in.v[i] = r < end ? *reinterpret_cast<const uint4 *>(v + (int64_t)r * p.v_stride + (tid & 7) * 8) : zero;
+    }
+    in.g = in.b = 0.0f;
+    if (tid < RK_C && t0 + tid < end) {
+        in.g = p.g[(int64_t)(t0 + tid) * p.n_head + h];
+        if (p.beta) in.b = p.beta[(int64_t)(t0 + tid) * p.n_head + h];
+    }
+}
+// The largest magnitude of eight bf16 values, as bits (a NaN is above infinity).
+__device__ __forceinline__ uint32_t max_bits(const uint4 &u) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) m = max(m, max(w[i] & 0x7fffu, w[i] >> 16 & 0x7fffu));
+    return m;
+}
+// Sixteen lanes hold a row: to f16, scaled by a power of two.  Returns the inverse scale.
+__device__ __forceinline__ float rk_row_f16(const uint4 &u, uint8_t *dst, bool &bad) {
+    uint32_t m = max_bits(u);
+#pragma unroll
+    for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    bad |= m >= 0x7f80u;
+    float inv;
+    const float s = pow2_scale<0>(__uint_as_float(m << 16), inv);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = pack_f16(__uint_as_float(w[i] << 16) * s, __uint_as_float(w[i] & 0xffff0000u) * s);
+    *reinterpret_cast<uint4 *>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+    return inv;
+}
+
+// One 16 x 8 block product of the inverse: D[16][8] += A[16][16] B[16][8], lane (r = lane / 2, half = lane % 2)
+// holding four columns of row r.
+__device__ __forceinline__ void rk_block(float (&d)[4], const float *a, const float *b, int lane) {
+    const float *ar = a + (lane >> 1) * RK_PITCH, *bc = b + (lane & 1) * 4;
+#pragma unroll
+    for (int k4 = 0; k4 < 4; k4++) {
+        const float4 x = *reinterpret_cast<const float4 *>(ar + 4 * k4);
+        const float xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float4 y = *reinterpret_cast<const float4 *>(bc + (4 * k4 + k) * RK_PITCH);
+            d[0] = fmaf(xs[k], y.x, d[0]);
+            d[1] = fmaf(xs[k], y.y, d[1]);
+            d[2] = fmaf(xs[k], y.z, d[2]);
+            d[3] = fmaf(xs[k], y.w, d[3]);
+        }
+    }
+}
+
+template <bool DELTA>
+__device__ __forceinline__ void rk_produce(const RecParams &p, uint8_t *sm, int h, int row0, int32_t beg, int32_t end) {
+    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int hk = h / (p.n_head / p.n_head_k);
+    const __nv_bfloat16 *kp = static_cast<const __nv_bfloat16 *>(p.k) + (int64_t)hk * REC_HD;
+    const __nv_bfloat16 *qp = static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)hk * REC_HD;
+    const __nv_bfloat16 *vp = static_cast<const __nv_bfloat16 *>(p.v) + (int64_t)h * REC_HD + row0;
+    float *As = reinterpret_cast<float *>(sm + RK_A), *Ts = reinterpret_cast<float *>(sm + RK_T);
+    float *gs = reinterpret_cast<float *>(sm + RK_SMALL), *bs = gs + RK_C, *Gh = bs + RK_C, *Gl = Gh + RK_C, *iK = Gl + RK_C,
+          *iQ = iK + RK_C;
+    const uint32_t smu = (uint32_t)__cvta_generic_to_shared(sm);
+    RkIn in;
+    rk_load(in, p, kp, qp, vp, h, beg, end, tid);
+    int c = 0;
+    for (int32_t t0 = beg; t0 < end; t0 += RK_C, c++) {
+        const int st = c & 1;
+        uint8_t *sg = sm + st * RK_STAGE;
+        const uint32_t su = smu + st * RK_STAGE;
+        float *cf = reinterpret_cast<float *>(sg + RK_COEF);
+        bar_sync(BAR_EMPTY + st, RK_THREADS);
+        bool bad = false;
+        if (tid == 0) cf[CF_N * RK_C + 1] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = 16 * i + (tid >> 4), ch = tid & 15;
+            const float ik = rk_row_f16(in.k[i], sg + RK_K + r * 256 + ((ch ^ (r & 7)) << 4), bad);
+            const float iq = rk_row_f16(in.q[i], sg + RK_Q + r * 256 + ((ch ^ (r & 7)) << 4), bad);
+            if (ch == 0) {
+                iK[r] = ik;
+                iQ[r] = iq;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int r = 32 * i + (tid >> 3), ch = tid & 7;
+            bad |= max_bits(in.v[i]) >= 0x7f80u;
+            *reinterpret_cast<uint4 *>(sg + RK_V + r * (RK_ROWS * 2) + ((ch ^ (r & 7)) << 4)) = in.v[i];
+        }
+        if (tid < RK_C) {
+            // below e^-128 = 0: the clamp keeps sums and differences finite
+            gs[tid] = fmaxf(in.g, -128.0f);
+            bs[tid] = in.b;
+            bad |= !(in.g <= 3.0e38f) || !(fabsf(in.b) <= 3.0e38f);
+        }
+        rk_load(in, p, kp, qp, vp, h, t0 + RK_C, end, tid);
+        bar_sync(BAR_PROD, RK_PROD);
+        if (bad) cf[CF_N * RK_C + 1] = 1.0f;
+        // scores: warps 0 .. 3 k k^T (delta rule), 4 .. 7 q k^T, 16 rows each, columns up to the diagonal
+        const int w = wid & 3;
+        const bool scores = wid >= 4;
+        float acc[8][4];
+#pragma unroll
+        for (int n = 0; n < 8; n++) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+        if (DELTA || scores) {
+            const int m = lane >> 3, r = lane & 7;
+            const uint32_t arow = su + (scores ? RK_Q : RK_K) + (16 * w + (m & 1) * 8 + r) * 256;
+            const uint32_t brow = su + RK_K + ((m >> 1) * 8 + r) * 256;
+#pragma unroll
+            for (int kk = 0; kk < 8; kk++) {
+                uint32_t a[4], b[4];
+                ldsm4(a, arow + (((2 * kk + (m >> 1)) ^ r) << 4));
+#pragma unroll
+                for (int np = 0; np < 4; np++)
+                    if (np <= w) {
+                        ldsm4(b, brow + np * 4096 + (((2 * kk + (m & 1)) ^ r) << 4));
+                        mma_f16(acc[2 * np], a, b[0], b[1]);
+                        mma_f16(acc[2 * np + 1], a, b[2], b[3]);
+                    }
+            }
+        }
+        if (wid == 0) {   // sums of g in 64 bits, two tokens per lane
+            const double g0 = gs[2 * lane], g1 = gs[2 * lane + 1];
+            double s = g0 + g1;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double up = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += up;
+            }
+            const double a = s - g1;
+            Gh[2 * lane] = (float)a;
+            Gl[2 * lane] = (float)(a - (double)(float)a);
+            Gh[2 * lane + 1] = (float)s;
+            Gl[2 * lane + 1] = (float)(s - (double)(float)s);
+        }
+        bar_sync(BAR_PROD, RK_PROD);
+        if (tid < RK_C) {
+            const float gam = __expf(Gh[tid]) * (1.0f + Gl[tid]);
+            const float end_g = __expf((Gh[RK_C - 1] - Gh[tid]) + (Gl[RK_C - 1] - Gl[tid]));
+            cf[CF_X * RK_C + tid] = -bs[tid] * gam * iK[tid];
+            cf[CF_V * RK_C + tid] = bs[tid];
+            cf[CF_Q1 * RK_C + tid] = p.scale * gam * iQ[tid];
+            cf[CF_W * RK_C + tid] = end_g * iK[tid];
+            if (tid == RK_C - 1) cf[CF_N * RK_C] = gam;
+        }
+        if (DELTA || scores) {
+            const int i0 = 16 * w + g, i1 = i0 + 8;
+            const float h0 = Gh[i0], l0 = Gl[i0], h1 = Gh[i1], l1 = Gl[i1];
+#pragma unroll
+            for (int n = 0; n < 8; n++)
+                if (n < 2 * (w + 1)) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int j = 8 * n + 2 * t + e;
+                        const float hj = Gh[j], lj = Gl[j], ik = iK[j];
+                        const float d0 = __expf((h0 - hj) + (l0 - lj)) * ik, d1 = __expf((h1 - hj) + (l1 - lj)) * ik;
+                        acc[n][e] = j <= i0 ? acc[n][e] * d0 : 0.0f;
+                        acc[n][2 + e] = j <= i1 ? acc[n][2 + e] * d1 : 0.0f;
+                    }
+                }
+            if (scores) {
+                float s0, s1, v0, v1;
+                row_scales(acc, s0, s1, v0, v1);
+#pragma unroll
+                for (int n = 0; n < 8; n++)
+                    if (n < 2 * (w + 1)) {
+                        *reinterpret_cast<uint32_t *>(sg + RK_P + i0 * 128 + ((n ^ (i0 & 7)) << 4) + t * 4) = pack_f16(acc[n][0] * s0, acc[n][1] * s0);
+                        *reinterpret_cast<uint32_t *>(sg + RK_P + i1 * 128 + ((n ^ (i1 & 7)) << 4) + t * 4) = pack_f16(acc[n][2] * s1, acc[n][3] * s1);
+                    }
+                if (t == 0) {
+                    cf[CF_Q2 * RK_C + i0] = p.scale * iQ[i0] * v0;
+                    cf[CF_Q2 * RK_C + i1] = p.scale * iQ[i1] * v1;
+                }
+            } else {
+                const float b0 = bs[i0] * iK[i0], b1 = bs[i1] * iK[i1];
+#pragma unroll
+                for (int n = 0; n < 8; n++)
+                    if (n < 2 * (w + 1)) {
+                        *reinterpret_cast<float2 *>(As + i0 * RK_PITCH + 8 * n + 2 * t) = make_float2(acc[n][0] * b0, acc[n][1] * b0);
+                        *reinterpret_cast<float2 *>(As + i1 * RK_PITCH + 8 * n + 2 * t) = make_float2(acc[n][2] * b1, acc[n][3] * b1);
+                    }
+            }
+        }
+        if (DELTA) {
+            bar_sync(BAR_PROD, RK_PROD);
+            // T's diagonal 16 x 16 blocks by forward substitution, a column per lane (warps 0 .. 3)
+            if (wid < 4 && lane < 16) {
+                const float *a = As + (16 * wid) * RK_PITCH + 16 * wid;
+                float *o = Ts + (16 * wid) * RK_PITCH + 16 * wid + lane;
+                float x[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float s = i == lane ? 1.0f : 0.0f;
+#pragma unroll
+                    for (int j = 0; j < i; j++) s = fmaf(-a[i * RK_PITCH + j], x[j], s);
+                    x[i] = s;
+                    o[i * RK_PITCH] = s;
+                }
+            }
+            bar_sync(BAR_PROD, RK_PROD);
+            // the blocks below, column by column: T_ij = -T_ii sum_{j <= k < i} A_ik T_kj; a warp takes 8 of a block
+            // column's 16 columns (it reads only what it wrote, and the diagonal)
+            const int jb = wid >> 1, half = (wid & 1) * 8;
+            for (int ib = jb + 1; ib < 4; ib++) {
+                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (int k = jb; k < ib; k++)
+                    rk_block(d, As + (16 * ib) * RK_PITCH + 16 * k, Ts + (16 * k) * RK_PITCH + 16 * jb + half, lane);
+                float *o = Ts + (16 * ib + (lane >> 1)) * RK_PITCH + 16 * jb + half + (lane & 1) * 4;
+                *reinterpret_cast<float4 *>(o) = make_float4(d[0], d[1], d[2], d[3]);
+                __syncwarp();
+                float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                rk_block(e, Ts + (16 * ib) * RK_PITCH + 16 * ib, Ts + (16 * ib) * RK_PITCH + 16 * jb + half, lane);
+                __syncwarp();
+                *reinterpret_cast<float4 *>(o) = make_float4(-e[0], -e[1], -e[2], -e[3]);
+                __syncwarp();
+            }
+            bar_sync(BAR_PROD, RK_PROD);
+            {   // T as two f16 terms of scaled rows; row tid / 4, columns 16 (tid % 4) ..: zero above the diagonal blocks
+                const int i = tid >> 2, j0 = (tid & 3) * 16;
+                float x[16];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float4 u = *reinterpret_cast<const float4 *>(Ts + i * RK_PITCH + j0 + 4 * k);
+                    const bool in_ = j0 <= (i & ~15);
+                    x[4 * k] = in_ ? u.x : 0.0f;
+                    x[4 * k + 1] = in_ ? u.y : 0.0f;
+                    x[4 * k + 2] = in_ ? u.z : 0.0f;
+                    x[4 * k + 3] = in_ ? u.w : 0.0f;
+                }
+                float mx = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 16; k++) mx = fmaxf(mx, fabsf(x[k]));
+                float inv;
+                const float s = pow2_scale<12>(quad_max(mx), inv);
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) split_f16(x[2 * k], x[2 * k + 1], s, hi[k], lo[k]);
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const int off = i * 128 + (((j0 / 8 + k) ^ (i & 7)) << 4);
+                    *reinterpret_cast<uint4 *>(sg + RK_TH + off) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
+                    *reinterpret_cast<uint4 *>(sg + RK_TL + off) = make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
+                }
+                if ((tid & 3) == 0) cf[CF_T * RK_C + i] = inv;
+            }
+        }
+        bar_arrive(BAR_FULL + st, RK_THREADS);
+    }
+}
+
+// A flagged chunk, token by token: S in the chain's registers, everything else from global memory.
+template <bool DELTA>
+__device__ __noinline__ void rk_serial(const RecParams &p, float (&S)[16][4], int h, int dv, int32_t t0, int32_t t1) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int hk = h / (p.n_head / p.n_head_k);
+    for (int32_t r = t0; r < t1; r++) {
+        const __nv_bfloat162 *k = reinterpret_cast<const __nv_bfloat162 *>(static_cast<const __nv_bfloat16 *>(p.k) + (int64_t)r * p.k_stride + hk * REC_HD);
+        const __nv_bfloat162 *q = reinterpret_cast<const __nv_bfloat162 *>(static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)r * p.q_stride + hk * REC_HD);
+        const __nv_bfloat16 *v = static_cast<const __nv_bfloat16 *>(p.v) + (int64_t)r * p.v_stride + h * REC_HD + dv;
+        const float eg = expf(p.g[(int64_t)r * p.n_head + h]);
+        float u0 = __bfloat162float(v[g]), u1 = __bfloat162float(v[g + 8]), d0 = 0.0f, d1 = 0.0f, o0 = 0.0f, o1 = 0.0f;
+#pragma unroll
+        for (int n = 0; n < 16; n++) {
+            const float2 kf = __bfloat1622float2(k[4 * n + t]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) S[n][e] *= eg;
+            d0 += S[n][0] * kf.x + S[n][1] * kf.y;
+            d1 += S[n][2] * kf.x + S[n][3] * kf.y;
+        }
+        if (DELTA) {
+            const float b = p.beta[(int64_t)r * p.n_head + h];
+            u0 = b * (u0 - quad_sum(d0));
+            u1 = b * (u1 - quad_sum(d1));
+        }
+#pragma unroll
+        for (int n = 0; n < 16; n++) {
+            const float2 kf = __bfloat1622float2(k[4 * n + t]), qf = __bfloat1622float2(q[4 * n + t]);
+            S[n][0] = fmaf(u0, kf.x, S[n][0]);
+            S[n][1] = fmaf(u0, kf.y, S[n][1]);
+            S[n][2] = fmaf(u1, kf.x, S[n][2]);
+            S[n][3] = fmaf(u1, kf.y, S[n][3]);
+            o0 += S[n][0] * qf.x + S[n][1] * qf.y;
+            o1 += S[n][2] * qf.x + S[n][3] * qf.y;
+        }
+        o0 = quad_sum(o0);
+        o1 = quad_sum(o1);
+        if (t == 0) {
+            __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(p.out) + ((int64_t)r * p.n_head + h) * REC_HD + dv;
+            o[g] = __float2bfloat16_rn(o0 * p.scale);
+            o[g + 8] = __float2bfloat16_rn(o1 * p.scale);
+        }
+    }
+}
+
+template <bool DELTA>
+__device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, int seq, int h, int row0, int32_t beg, int32_t end) {
+    const int lane = threadIdx.x & 31, wid = (threadIdx.x - RK_PROD) >> 5, g = lane >> 2, t = lane & 3;
+    const int m = lane >> 3, r = lane & 7;
+    const uint32_t smu = (uint32_t)__cvta_generic_to_shared(sm);
+    const int dv = row0 + 16 * wid;
+    float *S0 = reinterpret_cast<float *>(p.state + (int64_t)p.slot[seq] * p.slot_bytes) + ((int64_t)h * REC_HD + dv) * REC_HD;
+    const int n_chunks = (end - beg + RK_C - 1) / RK_C;
+    bar_arrive(BAR_EMPTY, RK_THREADS);
+    if (n_chunks > 1) bar_arrive(BAR_EMPTY + 1, RK_THREADS);
+    float S[16][4];   // rows dv + g and dv + g + 8, keys 8 n + 2 t, + 1
+#pragma unroll
+    for (int n = 0; n < 16; n++) {
+        const float2 a = *reinterpret_cast<const float2 *>(S0 + g * REC_HD + 8 * n + 2 * t);
+        const float2 b = *reinterpret_cast<const float2 *>(S0 + (g + 8) * REC_HD + 8 * n + 2 * t);
+        S[n][0] = a.x; S[n][1] = a.y; S[n][2] = b.x; S[n][3] = b.y;
+    }
+    for (int c = 0; c < n_chunks; c++) {
+        const int st = c & 1;
+        const int32_t t0 = beg + c * RK_C;
+        uint8_t *sg = sm + st * RK_STAGE;
+        const uint32_t su = smu + st * RK_STAGE;
+        const float *cf = reinterpret_cast<const float *>(sg + RK_COEF);
+        bar_sync(BAR_FULL + st, RK_THREADS);
+        if (cf[CF_N * RK_C + 1] != 0.0f) {
+            rk_serial<DELTA>(p, S, h, dv, t0, min(end, t0 + RK_C));
+            if (c + 2 < n_chunks) bar_arrive(BAR_EMPTY + st, RK_THREADS);
+            continue;
+        }
+        float s0, s1, is0, is1;
+        row_scales(S, s0, s1, is0, is1);
+        // X = S K^T, then R; or V
+        float X[8][4];
+#pragma unroll
+        for (int n = 0; n < 8; n++) X[n][0] = X[n][1] = X[n][2] = X[n][3] = 0.0f;
+        const uint32_t krow = su + ((m >> 1) * 8 + r) * 256;
+        if (DELTA) {
+#pragma unroll
+            for (int kk = 0; kk < 8; kk++) {
+                uint32_t hi[4], lo[4], b[4];
+                split_f16(S[2 * kk][0], S[2 * kk][1], s0, hi[0], lo[0]);
+                split_f16(S[2 * kk][2], S[2 * kk][3], s1, hi[1], lo[1]);
+                split_f16(S[2 * kk + 1][0], S[2 * kk + 1][1], s0, hi[2], lo[2]);
+                split_f16(S[2 * kk + 1][2], S[2 * kk + 1][3], s1, hi[3], lo[3]);
+#pragma unroll
+                for (int np = 0; np < 4; np++) {
+                    ldsm4(b, krow + RK_K + np * 4096 + (((2 * kk + (m & 1)) ^ r) << 4));
+                    mma_f16(X[2 * np], hi, b[0], b[1]);
+                    mma_f16(X[2 * np + 1], hi, b[2], b[3]);
+                    mma_f16(X[2 * np], lo, b[0], b[1]);
+                    mma_f16(X[2 * np + 1], lo, b[2], b[3]);
+                }
+            }
+        }
+        const uint32_t vrow = su + RK_V + ((m >> 1) * 8 + r) * (RK_ROWS * 2) + (((2 * wid + (m & 1)) ^ r) << 4);
+#pragma unroll
+        for (int np = 0; np < 4; np++) {
+            uint32_t v[4];
+            ldsm4t(v, vrow + np * 16 * (RK_ROWS * 2));
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                float *x = &X[2 * np + (k >> 1)][(k & 1) * 2];
+                const float v0 = __uint_as_float(v[k] << 16), v1 = __uint_as_float(v[k] & 0xffff0000u);
+                if (DELTA) {
+                    const float2 cx = *reinterpret_cast<const float2 *>(cf + CF_X * RK_C + 8 * (2 * np + (k >> 1)) + 2 * t);
+                    const float2 cv = *reinterpret_cast<const float2 *>(cf + CF_V * RK_C + 8 * (2 * np + (k >> 1)) + 2 * t);
+                    const float is = k & 1 ? is1 : is0;
+                    x[0] = fmaf(cx.x * is, x[0], cv.x * v0);
+                    x[1] = fmaf(cx.y * is, x[1], cv.y * v1);
+                } else {
+                    x[0] = v0;
+                    x[1] = v1;
+                }
+            }
+        }
+        const uint32_t trow = su + ((m >> 1) * 8 + r) * 128;   // T and P: rows 16 ip + .., chunks 2 jj + ..
+        if (DELTA) {   // U = R T^T
+            float r0, r1, ir0, ir1;
+            row_scales(X, r0, r1, ir0, ir1);
+            uint32_t hi[4][4], lo[4][4];
+#pragma unroll
+            for (int jj = 0; jj < 4; jj++) {
+                split_f16(X[2 * jj][0], X[2 * jj][1], r0, hi[jj][0], lo[jj][0]);
+                split_f16(X[2 * jj][2], X[2 * jj][3], r1, hi[jj][1], lo[jj][1]);
+                split_f16(X[2 * jj + 1][0], X[2 * jj + 1][1], r0, hi[jj][2], lo[jj][2]);
+                split_f16(X[2 * jj + 1][2], X[2 * jj + 1][3], r1, hi[jj][3], lo[jj][3]);
+            }
+#pragma unroll
+            for (int n = 0; n < 8; n++) X[n][0] = X[n][1] = X[n][2] = X[n][3] = 0.0f;
+#pragma unroll
+            for (int jj = 0; jj < 4; jj++)
+#pragma unroll
+                for (int ip = jj; ip < 4; ip++) {
+                    uint32_t bh[4], bl[4];
+                    ldsm4(bh, trow + RK_TH + ip * 2048 + (((2 * jj + (m & 1)) ^ r) << 4));
+                    ldsm4(bl, trow + RK_TL + ip * 2048 + (((2 * jj + (m & 1)) ^ r) << 4));
+                    mma_f16(X[2 * ip], hi[jj], bh[0], bh[1]);
+                    mma_f16(X[2 * ip + 1], hi[jj], bh[2], bh[3]);
+                    mma_f16(X[2 * ip], lo[jj], bh[0], bh[1]);
+                    mma_f16(X[2 * ip + 1], lo[jj], bh[2], bh[3]);
+                    mma_f16(X[2 * ip], hi[jj], bl[0], bl[1]);
+                    mma_f16(X[2 * ip + 1], hi[jj], bl[2], bl[3]);
+                }
+#pragma unroll
+            for (int n = 0; n < 8; n++) {
+                const float2 ct = *reinterpret_cast<const float2 *>(cf + CF_T * RK_C + 8 * n + 2 * t);
+                X[n][0] *= ct.x * ir0;
+                X[n][1] *= ct.y * ir0;
+                X[n][2] *= ct.x * ir1;
+                X[n][3] *= ct.y * ir1;
+            }
+        }
+        // O = S Q^T and P U: leading f16 terms alone
+        {
+            float u0, u1, iu0, iu1;
+            row_scales(X, u0, u1, iu0, iu1);
+            float O[8][4];
+#pragma unroll
+            for (int n = 0; n < 8; n++) O[n][0] = O[n][1] = O[n][2] = O[n][3] = 0.0f;
+#pragma unroll
+            for (int kk = 0; kk < 8; kk++) {
+                uint32_t a[4], b[4];
+                a[0] = pack_f16(S[2 * kk][0] * s0, S[2 * kk][1] * s0);
+                a[1] = pack_f16(S[2 * kk][2] * s1, S[2 * kk][3] * s1);
+                a[2] = pack_f16(S[2 * kk + 1][0] * s0, S[2 * kk + 1][1] * s0);
+                a[3] = pack_f16(S[2 * kk + 1][2] * s1, S[2 * kk + 1][3] * s1);
+#pragma unroll
+                for (int np = 0; np < 4; np++) {
+                    ldsm4(b, krow + RK_Q + np * 4096 + (((2 * kk + (m & 1)) ^ r) << 4));
+                    mma_f16(O[2 * np], a, b[0], b[1]);
+                    mma_f16(O[2 * np + 1], a, b[2], b[3]);
+                }
+            }
+            uint32_t ua[4][4];
+#pragma unroll
+            for (int jj = 0; jj < 4; jj++) {
+                ua[jj][0] = pack_f16(X[2 * jj][0] * u0, X[2 * jj][1] * u0);
+                ua[jj][1] = pack_f16(X[2 * jj][2] * u1, X[2 * jj][3] * u1);
+                ua[jj][2] = pack_f16(X[2 * jj + 1][0] * u0, X[2 * jj + 1][1] * u0);
+                ua[jj][3] = pack_f16(X[2 * jj + 1][2] * u1, X[2 * jj + 1][3] * u1);
+            }
+#pragma unroll
+            for (int ip = 0; ip < 4; ip++) {
+                float d[2][4] = {};
+#pragma unroll
+                for (int jj = 0; jj <= ip; jj++) {
+                    uint32_t b[4];
+                    ldsm4(b, trow + RK_P + ip * 2048 + (((2 * jj + (m & 1)) ^ r) << 4));
+                    mma_f16(d[0], ua[jj], b[0], b[1]);
+                    mma_f16(d[1], ua[jj], b[2], b[3]);
+                }
+                uint32_t o[4];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const int n = 2 * ip + k;
+                    const float2 q1 = *reinterpret_cast<const float2 *>(cf + CF_Q1 * RK_C + 8 * n + 2 * t);
+                    const float2 q2 = *reinterpret_cast<const float2 *>(cf + CF_Q2 * RK_C + 8 * n + 2 * t);
+                    const __nv_bfloat162 a = __floats2bfloat162_rn(fmaf(q1.x * is0, O[n][0], q2.x * iu0 * d[k][0]),
+                                                                   fmaf(q1.y * is0, O[n][1], q2.y * iu0 * d[k][1]));
+                    const __nv_bfloat162 b = __floats2bfloat162_rn(fmaf(q1.x * is1, O[n][2], q2.x * iu1 * d[k][2]),
+                                                                   fmaf(q1.y * is1, O[n][3], q2.y * iu1 * d[k][3]));
+                    o[2 * k] = *reinterpret_cast<const uint32_t *>(&a);
+                    o[2 * k + 1] = *reinterpret_cast<const uint32_t *>(&b);
+                }
+                stsm4t(vrow + ip * 16 * (RK_ROWS * 2), o);   // over the warp's own columns of v
+            }
+        }
+        __syncwarp();
+        {
+            __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out) + ((int64_t)t0 * p.n_head + h) * REC_HD + dv + (lane & 1) * 8;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int tok = 16 * i + (lane >> 1);
+                const uint4 u = *reinterpret_cast<const uint4 *>(sg + RK_V + tok * (RK_ROWS * 2) + (((2 * wid + (lane & 1)) ^ (tok & 7)) << 4));
+                if (t0 + tok < end) *reinterpret_cast<uint4 *>(out + (int64_t)tok * p.n_head * REC_HD) = u;
+            }
+        }
+        // S = e^(G_C) S + (w U) K
+        {
+            float u0, u1, iu0, iu1;
+            uint32_t hi[4][4], lo[4][4];
+#pragma unroll
+            for (int n = 0; n < 8; n++) {
+                const float2 cw = *reinterpret_cast<const float2 *>(cf + CF_W * RK_C + 8 * n + 2 * t);
+                X[n][0] *= cw.x;
+                X[n][1] *= cw.y;
+                X[n][2] *= cw.x;
+                X[n][3] *= cw.y;
+            }
+            row_scales(X, u0, u1, iu0, iu1);
+#pragma unroll
+            for (int jj = 0; jj < 4; jj++) {
+                split_f16(X[2 * jj][0], X[2 * jj][1], u0, hi[jj][0], lo[jj][0]);
+                split_f16(X[2 * jj][2], X[2 * jj][3], u1, hi[jj][1], lo[jj][1]);
+                split_f16(X[2 * jj + 1][0], X[2 * jj + 1][1], u0, hi[jj][2], lo[jj][2]);
+                split_f16(X[2 * jj + 1][2], X[2 * jj + 1][3], u1, hi[jj][3], lo[jj][3]);
+            }
+            const float eg = cf[CF_N * RK_C];
+            const uint32_t ktrow = su + RK_K + ((m & 1) * 8 + r) * 256;
+#pragma unroll
+            for (int dg = 0; dg < 4; dg++) {
+                float d[4][4] = {};
+#pragma unroll
+                for (int jj = 0; jj < 4; jj++) {
+                    uint32_t b0[4], b1[4];
+                    ldsm4t(b0, ktrow + jj * 4096 + (((4 * dg + (m >> 1)) ^ r) << 4));
+                    ldsm4t(b1, ktrow + jj * 4096 + (((4 * dg + 2 + (m >> 1)) ^ r) << 4));
+                    mma_f16(d[0], hi[jj], b0[0], b0[1]);
+                    mma_f16(d[1], hi[jj], b0[2], b0[3]);
+                    mma_f16(d[2], hi[jj], b1[0], b1[1]);
+                    mma_f16(d[3], hi[jj], b1[2], b1[3]);
+                    mma_f16(d[0], lo[jj], b0[0], b0[1]);
+                    mma_f16(d[1], lo[jj], b0[2], b0[3]);
+                    mma_f16(d[2], lo[jj], b1[0], b1[1]);
+                    mma_f16(d[3], lo[jj], b1[2], b1[3]);
+                }
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    S[4 * dg + n][0] = fmaf(eg, S[4 * dg + n][0], iu0 * d[n][0]);
+                    S[4 * dg + n][1] = fmaf(eg, S[4 * dg + n][1], iu0 * d[n][1]);
+                    S[4 * dg + n][2] = fmaf(eg, S[4 * dg + n][2], iu1 * d[n][2]);
+                    S[4 * dg + n][3] = fmaf(eg, S[4 * dg + n][3], iu1 * d[n][3]);
+                }
+            }
+        }
+        if (c + 2 < n_chunks) bar_arrive(BAR_EMPTY + st, RK_THREADS);
+    }
+#pragma unroll
+    for (int n = 0; n < 16; n++) {
+        *reinterpret_cast<float2 *>(S0 + g * REC_HD + 8 * n + 2 * t) = make_float2(S[n][0], S[n][1]);
+        *reinterpret_cast<float2 *>(S0 + (g + 8) * REC_HD + 8 * n + 2 * t) = make_float2(S[n][2], S[n][3]);
+    }
+}
+
+template <bool DELTA>
+__global__ void __launch_bounds__(RK_THREADS, 1) k_rec_chunk(const __grid_constant__ RecParams p) {
+    extern __shared__ __align__(1024) uint8_t rk_sm[];
+    const int seq = blockIdx.z, h = blockIdx.y, row0 = blockIdx.x * RK_ROWS;
+    const int32_t beg = p.cu[seq], end = p.cu[seq + 1];
+    if (beg < 0 || end > p.n_rows || beg > end) {
+        if (threadIdx.x == 0) atomicOr(p.status, ST_BAD_INDEX);
+        return;
+    }
+    if (beg == end) return;
+    if (threadIdx.x < RK_PROD) rk_produce<DELTA>(p, rk_sm, h, row0, beg, end);
+    else rk_chain<DELTA>(p, rk_sm, seq, h, row0, beg, end);
+}
+
 cudaError_t launch_rec_step(const RecParams &p, cudaStream_t st) {
     k_rec_serial<float><<<dim3(REC_HD / RT_ROWS, p.n_head, p.n_seq), RT_THREADS, 0, st>>>(p);
     count_launches(1);
@@ -327,7 +985,10 @@ cudaError_t launch_rec_step(const RecParams &p, cudaStream_t st) {
 }
 
 cudaError_t launch_rec_chunk(const RecParams &p, cudaStream_t st) {
-    k_rec_serial<__nv_bfloat16><<<dim3(REC_HD / RT_ROWS, p.n_head, p.n_seq), RT_THREADS, 0, st>>>(p);
+    auto *k = p.beta ? k_rec_chunk<true> : k_rec_chunk<false>;
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, RK_SMEM);
+    if (e != cudaSuccess) return e;
+    k<<<dim3(REC_HD / RK_ROWS, p.n_head, p.n_seq), RK_THREADS, RK_SMEM, st>>>(p);
     count_launches(1);
     return cudaGetLastError();
 }
