@@ -350,12 +350,13 @@ __global__ void __launch_bounds__(RT_THREADS) k_rec_serial(const __grid_constant
 constexpr int RK_C = 64, RK_NW = 4, RK_PROD = 256, RK_THREADS = RK_PROD + RK_NW * 32;
 constexpr int RK_ROWS = RK_NW * 16;
 constexpr int RK_K = 0, RK_Q = 16384, RK_P = 32768, RK_TH = 40960, RK_TL = 49152, RK_V = 57344;
-constexpr int RK_COEF = RK_V + RK_C * RK_ROWS * 2;      // six arrays of RK_C floats, then e^(G_C) and the flag
-enum { CF_X, CF_V, CF_T, CF_Q1, CF_Q2, CF_W, CF_N };
+constexpr int RK_COEF = RK_V + RK_C * RK_ROWS * 2;      // CF_N arrays of RK_C floats, then e^(G_C) and the flag
+enum { CF_X, CF_V, CF_T, CF_Q1, CF_Q2, CF_W, CF_K, CF_B, CF_N };
 constexpr int RK_STAGE = RK_COEF + CF_N * RK_C * 4 + 128;
-constexpr int RK_PITCH = 68;                            // floats per row of the producers' triangular matrices
+constexpr int RK_PITCH = 36;                            // floats per row of the 32 x 32 triangular blocks
 constexpr int RK_A = 2 * RK_STAGE, RK_T = RK_A + RK_C * RK_PITCH * 4, RK_SMALL = RK_T + RK_C * RK_PITCH * 4;
 constexpr int RK_SMEM = RK_SMALL + 6 * RK_C * 4;
+constexpr int RK_PROD_REGS = 104, RK_CHAIN_REGS = 240;  // of 168 at launch: 256 x 104 + 128 x 240 <= 384 x 168
 enum { BAR_FULL = 1, BAR_EMPTY = 3, BAR_PROD = 5 };
 
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
@@ -417,89 +418,74 @@ __device__ __forceinline__ void row_scales(const float (&x)[N][4], float &s0, fl
     s1 = pow2_scale<12>(quad_max(m1), i1);
 }
 
-// The chunk's inputs of a producer thread, loaded one chunk ahead: 4 x 16 bytes of k and of q (rows
-// 16 p + tid / 16, chunk tid % 16), 2 of v (rows 32 p + tid / 8, chunk tid % 8), g and beta of token tid.
-struct RkIn {
-    uint4 k[4], q[4], v[2];
-    float g, b;
-};
-__device__ __forceinline__ void rk_load(RkIn &in, const RecParams &p, const __nv_bfloat16 *k, const __nv_bfloat16 *q,
-                                        const __nv_bfloat16 *v, int h, int32_t t0, int32_t end, int tid) {
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int32_t r = t0 + 16 * i + (tid >> 4);
-        const bool ok = r < end;
-        in.k[i] = ok ? *reinterpret_cast<const uint4 *>(k + (int64_t)r * p.k_stride + (tid & 15) * 8) : zero;
-        in.q[i] = ok ? *reinterpret_cast<const uint4 *>(q + (int64_t)r * p.q_stride + (tid & 15) * 8) : zero;
-    }
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int32_t r = t0 + 32 * i + (tid >> 3);
-        in.v[i] = r < end ? *reinterpret_cast<const uint4 *>(v + (int64_t)r * p.v_stride + (tid & 7) * 8) : zero;
-    }
-    in.g = in.b = 0.0f;
-    if (tid < RK_C && t0 + tid < end) {
-        in.g = p.g[(int64_t)(t0 + tid) * p.n_head + h];
-        if (p.beta) in.b = p.beta[(int64_t)(t0 + tid) * p.n_head + h];
-    }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
-// The largest magnitude of eight bf16 values, as bits (a NaN is above infinity).
-__device__ __forceinline__ uint32_t max_bits(const uint4 &u) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ void rk_cp16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// Sixteen words of bf16 pairs, four lanes holding a row of 128: to f16, the row scaled by a power of two to
+// [1, 2).  dst: the row; lane l holds its 16-byte chunks l, l + 4, l + 8, l + 12.  Returns the inverse scale.
+__device__ __forceinline__ float rk_row_f16(const uint4 (&u)[4], uint8_t *dst, int l, int sw, bool &bad) {
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) m = max(m, max(w[i] & 0x7fffu, w[i] >> 16 & 0x7fffu));
-    return m;
-}
-// Sixteen lanes hold a row: to f16, scaled by a power of two.  Returns the inverse scale.
-__device__ __forceinline__ float rk_row_f16(const uint4 &u, uint8_t *dst, bool &bad) {
-    uint32_t m = max_bits(u);
-#pragma unroll
-    for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int i = 0; i < 4; i++) {
+        m = __vmaxu2(m, u[i].x & 0x7fff7fffu);
+        m = __vmaxu2(m, u[i].y & 0x7fff7fffu);
+        m = __vmaxu2(m, u[i].z & 0x7fff7fffu);
+        m = __vmaxu2(m, u[i].w & 0x7fff7fffu);
+    }
+    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    m = max(m & 0xffffu, m >> 16);           // bits of the largest magnitude; a NaN is above infinity
     bad |= m >= 0x7f80u;
     float inv;
     const float s = pow2_scale<0>(__uint_as_float(m << 16), inv);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    uint32_t o[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) o[i] = pack_f16(__uint_as_float(w[i] << 16) * s, __uint_as_float(w[i] & 0xffff0000u) * s);
-    *reinterpret_cast<uint4 *>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
-    return inv;
-}
-
-// One 16 x 8 block product of the inverse: D[16][8] += A[16][16] B[16][8], lane (r = lane / 2, half = lane % 2)
-// holding four columns of row r.
-__device__ __forceinline__ void rk_block(float (&d)[4], const float *a, const float *b, int lane) {
-    const float *ar = a + (lane >> 1) * RK_PITCH, *bc = b + (lane & 1) * 4;
+    for (int i = 0; i < 4; i++) {
+        const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+        uint32_t o[4];
 #pragma unroll
-    for (int k4 = 0; k4 < 4; k4++) {
-        const float4 x = *reinterpret_cast<const float4 *>(ar + 4 * k4);
-        const float xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const float4 y = *reinterpret_cast<const float4 *>(bc + (4 * k4 + k) * RK_PITCH);
-            d[0] = fmaf(xs[k], y.x, d[0]);
-            d[1] = fmaf(xs[k], y.y, d[1]);
-            d[2] = fmaf(xs[k], y.z, d[2]);
-            d[3] = fmaf(xs[k], y.w, d[3]);
-        }
+        for (int j = 0; j < 4; j++) o[j] = pack_f16(__uint_as_float(w[j] << 16) * s, __uint_as_float(w[j] & 0xffff0000u) * s);
+        *reinterpret_cast<uint4 *>(dst + (((l + 4 * i) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
     }
+    return inv;
 }
 
 template <bool DELTA>
 __device__ __forceinline__ void rk_produce(const RecParams &p, uint8_t *sm, int h, int row0, int32_t beg, int32_t end) {
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
     const int hk = h / (p.n_head / p.n_head_k);
-    const __nv_bfloat16 *kp = static_cast<const __nv_bfloat16 *>(p.k) + (int64_t)hk * REC_HD;
-    const __nv_bfloat16 *qp = static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)hk * REC_HD;
-    const __nv_bfloat16 *vp = static_cast<const __nv_bfloat16 *>(p.v) + (int64_t)h * REC_HD + row0;
     float *As = reinterpret_cast<float *>(sm + RK_A), *Ts = reinterpret_cast<float *>(sm + RK_T);
     float *gs = reinterpret_cast<float *>(sm + RK_SMALL), *bs = gs + RK_C, *Gh = bs + RK_C, *Gl = Gh + RK_C, *iK = Gl + RK_C,
           *iQ = iK + RK_C;
     const uint32_t smu = (uint32_t)__cvta_generic_to_shared(sm);
-    RkIn in;
-    rk_load(in, p, kp, qp, vp, h, beg, end, tid);
+    // This thread's row of k and q (a permutation within eight: the two rows of eight lanes differ in bit 2, so
+    // their swizzled 16-byte stores meet different banks) and its rows of v.
+    const int x = tid >> 2, row = (x & ~7) | ((x & 1) << 2) | ((x >> 1) & 3);
+    const __nv_bfloat16 *kp = static_cast<const __nv_bfloat16 *>(p.k) + (int64_t)(beg + row) * p.k_stride + (int64_t)hk * REC_HD + t * 8;
+    const __nv_bfloat16 *qp = static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)(beg + row) * p.q_stride + (int64_t)hk * REC_HD + t * 8;
+    const __nv_bfloat16 *vp = static_cast<const __nv_bfloat16 *>(p.v) + (int64_t)(beg + (tid >> 3)) * p.v_stride + (int64_t)h * REC_HD + row0 + (tid & 7) * 8;
+    uint4 ku[4], qu[4];
+    float gu = 0.0f, bu = 0.0f;
+    auto load = [&](int32_t t0) {
+        const bool ok = t0 + row < end;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            ku[i] = ok ? *reinterpret_cast<const uint4 *>(kp + 32 * i) : make_uint4(0, 0, 0, 0);
+            qu[i] = ok ? *reinterpret_cast<const uint4 *>(qp + 32 * i) : make_uint4(0, 0, 0, 0);
+        }
+        kp += RK_C * p.k_stride;
+        qp += RK_C * p.q_stride;
+        gu = bu = 0.0f;
+        if (tid < RK_C && t0 + tid < end) {
+            gu = p.g[(int64_t)(t0 + tid) * p.n_head + h];
+            if (DELTA) bu = p.beta[(int64_t)(t0 + tid) * p.n_head + h];
+        }
+    };
+    load(beg);
     int c = 0;
     for (int32_t t0 = beg; t0 < end; t0 += RK_C, c++) {
         const int st = c & 1;
@@ -507,218 +493,221 @@ __device__ __forceinline__ void rk_produce(const RecParams &p, uint8_t *sm, int 
         const uint32_t su = smu + st * RK_STAGE;
         float *cf = reinterpret_cast<float *>(sg + RK_COEF);
         bar_sync(BAR_EMPTY + st, RK_THREADS);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {   // v as it is, zeros behind the sequence
+            const int r = 32 * i + (tid >> 3), ch = tid & 7;
+            const uint32_t off = RK_V + r * (RK_ROWS * 2) + ((ch ^ (r & 7)) << 4);
+            if (t0 + r < end) rk_cp16(su + off, vp + 32 * i * p.v_stride);
+            else *reinterpret_cast<uint4 *>(sg + off) = make_uint4(0, 0, 0, 0);
+        }
+        vp += RK_C * p.v_stride;
         bool bad = false;
         if (tid == 0) cf[CF_N * RK_C + 1] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = 16 * i + (tid >> 4), ch = tid & 15;
-            const float ik = rk_row_f16(in.k[i], sg + RK_K + r * 256 + ((ch ^ (r & 7)) << 4), bad);
-            const float iq = rk_row_f16(in.q[i], sg + RK_Q + r * 256 + ((ch ^ (r & 7)) << 4), bad);
-            if (ch == 0) {
-                iK[r] = ik;
-                iQ[r] = iq;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int r = 32 * i + (tid >> 3), ch = tid & 7;
-            bad |= max_bits(in.v[i]) >= 0x7f80u;
-            *reinterpret_cast<uint4 *>(sg + RK_V + r * (RK_ROWS * 2) + ((ch ^ (r & 7)) << 4)) = in.v[i];
+        const float ik = rk_row_f16(ku, sg + RK_K + row * 256, t, row & 7, bad);
+        const float iq = rk_row_f16(qu, sg + RK_Q + row * 256, t, row & 7, bad);
+        if (t == 0) {
+            iK[row] = ik;
+            iQ[row] = iq;
         }
         if (tid < RK_C) {
-            // below e^-128 = 0: the clamp keeps sums and differences finite
-            gs[tid] = fmaxf(in.g, -128.0f);
-            bs[tid] = in.b;
-            bad |= !(in.g <= 3.0e38f) || !(fabsf(in.b) <= 3.0e38f);
+            // in base 2; below 2^-184 = 0: the clamp keeps sums and differences finite.  A growing state
+            // (g > 0) would leave the range of the f16 scores: flagged, as what is not finite
+            gs[tid] = fmaxf(gu, -128.0f) * 1.4426950408889634f;
+            bs[tid] = bu;
+            bad |= !(gu <= 0.0f) || !(fabsf(bu) <= 3.0e38f);
         }
-        rk_load(in, p, kp, qp, vp, h, t0 + RK_C, end, tid);
+        load(t0 + RK_C);
         bar_sync(BAR_PROD, RK_PROD);
         if (bad) cf[CF_N * RK_C + 1] = 1.0f;
-        // scores: warps 0 .. 3 k k^T (delta rule), 4 .. 7 q k^T, 16 rows each, columns up to the diagonal
-        const int w = wid & 3;
-        const bool scores = wid >= 4;
-        float acc[8][4];
-#pragma unroll
-        for (int n = 0; n < 8; n++) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
-        if (DELTA || scores) {
-            const int m = lane >> 3, r = lane & 7;
-            const uint32_t arow = su + (scores ? RK_Q : RK_K) + (16 * w + (m & 1) * 8 + r) * 256;
-            const uint32_t brow = su + RK_K + ((m >> 1) * 8 + r) * 256;
-#pragma unroll
-            for (int kk = 0; kk < 8; kk++) {
-                uint32_t a[4], b[4];
-                ldsm4(a, arow + (((2 * kk + (m >> 1)) ^ r) << 4));
-#pragma unroll
-                for (int np = 0; np < 4; np++)
-                    if (np <= w) {
-                        ldsm4(b, brow + np * 4096 + (((2 * kk + (m & 1)) ^ r) << 4));
-                        mma_f16(acc[2 * np], a, b[0], b[1]);
-                        mma_f16(acc[2 * np + 1], a, b[2], b[3]);
-                    }
-            }
-        }
-        if (wid == 0) {   // sums of g in 64 bits, two tokens per lane
-            const double g0 = gs[2 * lane], g1 = gs[2 * lane + 1];
-            double s = g0 + g1;
+        if (wid == 7) {
+            // sums of g as pairs of floats (two-sum at each step), two tokens per lane
+            const float g0 = gs[2 * lane], g1 = gs[2 * lane + 1];
+            float hi = g0 + g1, lo = (g0 - (hi - (hi - g0))) + (g1 - (hi - g0));
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const double up = __shfl_up_sync(0xffffffffu, s, o);
-                if (lane >= o) s += up;
+                const float uh = __shfl_up_sync(0xffffffffu, hi, o), ul = __shfl_up_sync(0xffffffffu, lo, o);
+                const float s = hi + uh, b = s - hi;
+                const float e = (hi - (s - b)) + (uh - b) + (lo + ul);
+                if (lane >= o) {
+                    hi = s + e;
+                    lo = e - (hi - s);
+                }
             }
-            const double a = s - g1;
-            Gh[2 * lane] = (float)a;
-            Gl[2 * lane] = (float)(a - (double)(float)a);
-            Gh[2 * lane + 1] = (float)s;
-            Gl[2 * lane + 1] = (float)(s - (double)(float)s);
+            Gh[2 * lane + 1] = hi;
+            Gl[2 * lane + 1] = lo;
+            const float s = hi - g1, b = s - hi;
+            const float e = (hi - (s - b)) + (-g1 - b) + lo;
+            Gh[2 * lane] = s + e;
+            Gl[2 * lane] = e - ((s + e) - s);
+        }
+        // Scores, in 16 x 16 tiles on and below the diagonal: ten of q k^T, then (delta rule) ten of k k^T, spread
+        // over the warps; warp 7 has the sums of g and the fewest.
+        constexpr int NT = DELTA ? 20 : 10, PER = DELTA ? 3 : 2;
+        float acc[PER][2][4];
+        uint32_t arow[PER], brow[PER];
+        const int m = lane >> 3, r = lane & 7;
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            const int id = min(wid + 8 * k, NT - 1), tt = id % 10, ib = tt < 1 ? 0 : tt < 3 ? 1 : tt < 6 ? 2 : 3, jb = tt - ib * (ib + 1) / 2;
+            arow[k] = su + (id < 10 ? RK_Q : RK_K) + (16 * ib + (m & 1) * 8 + r) * 256;
+            brow[k] = su + RK_K + (16 * jb + (m >> 1) * 8 + r) * 256;
+#pragma unroll
+            for (int n = 0; n < 2; n++) acc[k][n][0] = acc[k][n][1] = acc[k][n][2] = acc[k][n][3] = 0.0f;
+        }
+#pragma unroll
+        for (int kk = 0; kk < 8; kk++) {
+#pragma unroll
+            for (int k = 0; k < PER; k++)
+                if (8 * k + 8 <= NT || wid + 8 * k < NT) {
+                    uint32_t a[4], b[4];
+                    ldsm4(a, arow[k] + (((2 * kk + (m >> 1)) ^ r) << 4));
+                    ldsm4(b, brow[k] + (((2 * kk + (m & 1)) ^ r) << 4));
+                    mma_f16(acc[k][0], a, b[0], b[1]);
+                    mma_f16(acc[k][1], a, b[2], b[3]);
+                }
         }
         bar_sync(BAR_PROD, RK_PROD);
         if (tid < RK_C) {
-            const float gam = __expf(Gh[tid]) * (1.0f + Gl[tid]);
-            const float end_g = __expf((Gh[RK_C - 1] - Gh[tid]) + (Gl[RK_C - 1] - Gl[tid]));
+            const float gam = ex2(Gh[tid]) * fmaf(Gl[tid], 0.6931471805599453f, 1.0f);
+            const float end_g = ex2((Gh[RK_C - 1] - Gh[tid]) + (Gl[RK_C - 1] - Gl[tid]));
             cf[CF_X * RK_C + tid] = -bs[tid] * gam * iK[tid];
             cf[CF_V * RK_C + tid] = bs[tid];
             cf[CF_Q1 * RK_C + tid] = p.scale * gam * iQ[tid];
-            cf[CF_W * RK_C + tid] = end_g * iK[tid];
+            cf[CF_Q2 * RK_C + tid] = p.scale * iQ[tid];
+            cf[CF_W * RK_C + tid] = end_g;
+            cf[CF_K * RK_C + tid] = iK[tid];
+            cf[CF_B * RK_C + tid] = -bs[tid] * iK[tid];
             if (tid == RK_C - 1) cf[CF_N * RK_C] = gam;
         }
-        if (DELTA || scores) {
-            const int i0 = 16 * w + g, i1 = i0 + 8;
-            const float h0 = Gh[i0], l0 = Gl[i0], h1 = Gh[i1], l1 = Gl[i1];
 #pragma unroll
-            for (int n = 0; n < 8; n++)
-                if (n < 2 * (w + 1)) {
+        for (int k = 0; k < PER; k++)
+            if (8 * k + 8 <= NT || wid + 8 * k < NT) {
+                const int id = wid + 8 * k, tt = id % 10, ib = tt < 1 ? 0 : tt < 3 ? 1 : tt < 6 ? 2 : 3, jb = tt - ib * (ib + 1) / 2;
+                const int i0 = 16 * ib + g, i1 = i0 + 8;
+                const float h0 = Gh[i0], l0 = Gl[i0], h1 = Gh[i1], l1 = Gl[i1];
+                const int s0 = i0 & 7;
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int j = 8 * n + 2 * t + e;
-                        const float hj = Gh[j], lj = Gl[j], ik = iK[j];
-                        const float d0 = __expf((h0 - hj) + (l0 - lj)) * ik, d1 = __expf((h1 - hj) + (l1 - lj)) * ik;
-                        acc[n][e] = j <= i0 ? acc[n][e] * d0 : 0.0f;
-                        acc[n][2 + e] = j <= i1 ? acc[n][2 + e] * d1 : 0.0f;
+                for (int n = 0; n < 2; n++) {
+                    const int j = 16 * jb + 8 * n + 2 * t;
+                    const float2 hj = *reinterpret_cast<const float2 *>(Gh + j), lj = *reinterpret_cast<const float2 *>(Gl + j);
+                    float *a = acc[k][n];
+                    a[0] *= ex2((h0 - hj.x) + (l0 - lj.x));
+                    a[1] *= ex2((h0 - hj.y) + (l0 - lj.y));
+                    a[2] *= ex2((h1 - hj.x) + (l1 - lj.x));
+                    a[3] *= ex2((h1 - hj.y) + (l1 - lj.y));
+                    if (ib == jb) {
+                        a[0] = j <= i0 ? a[0] : 0.0f;
+                        a[1] = j < i0 ? a[1] : 0.0f;
+                        a[2] = j <= i1 ? a[2] : 0.0f;
+                        a[3] = j < i1 ? a[3] : 0.0f;
+                    }
+                    const int off = i0 * 128 + (((2 * jb + n) ^ s0) << 4) + t * 4;   // row i1: 8 rows below, the same swizzle
+                    if (id < 10) {
+                        *reinterpret_cast<uint32_t *>(sg + RK_P + off) = pack_f16(a[0], a[1]);
+                        *reinterpret_cast<uint32_t *>(sg + RK_P + off + 1024) = pack_f16(a[2], a[3]);
+                    } else if (ib >= 2 && jb < 2) {   // A's lower left 32 x 32 quarter, |.| <= 512 without k's scales and beta
+                        uint32_t hi, lo;
+                        split_f16(a[0], a[1], 1.0f, hi, lo);
+                        *reinterpret_cast<uint32_t *>(sg + RK_TH + off) = hi;
+                        *reinterpret_cast<uint32_t *>(sg + RK_TL + off) = lo;
+                        split_f16(a[2], a[3], 1.0f, hi, lo);
+                        *reinterpret_cast<uint32_t *>(sg + RK_TH + off + 1024) = hi;
+                        *reinterpret_cast<uint32_t *>(sg + RK_TL + off + 1024) = lo;
+                    } else {
+                        const float b0 = -bs[i0] * iK[i0], b1 = -bs[i1] * iK[i1];
+                        const float2 kj = *reinterpret_cast<const float2 *>(iK + j);
+                        float *o = As + i0 * RK_PITCH + (j & 31);
+                        *reinterpret_cast<float2 *>(o) = make_float2(a[0] * b0 * kj.x, a[1] * b0 * kj.y);
+                        *reinterpret_cast<float2 *>(o + 8 * RK_PITCH) = make_float2(a[2] * b1 * kj.x, a[3] * b1 * kj.y);
                     }
                 }
-            if (scores) {
-                float s0, s1, v0, v1;
-                row_scales(acc, s0, s1, v0, v1);
-#pragma unroll
-                for (int n = 0; n < 8; n++)
-                    if (n < 2 * (w + 1)) {
-                        *reinterpret_cast<uint32_t *>(sg + RK_P + i0 * 128 + ((n ^ (i0 & 7)) << 4) + t * 4) = pack_f16(acc[n][0] * s0, acc[n][1] * s0);
-                        *reinterpret_cast<uint32_t *>(sg + RK_P + i1 * 128 + ((n ^ (i1 & 7)) << 4) + t * 4) = pack_f16(acc[n][2] * s1, acc[n][3] * s1);
-                    }
-                if (t == 0) {
-                    cf[CF_Q2 * RK_C + i0] = p.scale * iQ[i0] * v0;
-                    cf[CF_Q2 * RK_C + i1] = p.scale * iQ[i1] * v1;
-                }
-            } else {
-                const float b0 = bs[i0] * iK[i0], b1 = bs[i1] * iK[i1];
-#pragma unroll
-                for (int n = 0; n < 8; n++)
-                    if (n < 2 * (w + 1)) {
-                        *reinterpret_cast<float2 *>(As + i0 * RK_PITCH + 8 * n + 2 * t) = make_float2(acc[n][0] * b0, acc[n][1] * b0);
-                        *reinterpret_cast<float2 *>(As + i1 * RK_PITCH + 8 * n + 2 * t) = make_float2(acc[n][2] * b1, acc[n][3] * b1);
-                    }
             }
-        }
         if (DELTA) {
             bar_sync(BAR_PROD, RK_PROD);
-            // T's diagonal 16 x 16 blocks by forward substitution, a column per lane (warps 0 .. 3)
-            if (wid < 4 && lane < 16) {
-                const float *a = As + (16 * wid) * RK_PITCH + 16 * wid;
-                float *o = Ts + (16 * wid) * RK_PITCH + 16 * wid + lane;
-                float x[16];
+            // T's two diagonal 32 x 32 blocks by forward substitution, one warp each, a column per lane:
+            // x_i = [i = column] - sum_{j < i} A_ij x_j   (As holds -A)
+            if (wid < 2) {
+                const float *a = As + 32 * wid * RK_PITCH;
+                float *o = Ts + 32 * wid * RK_PITCH + lane;
+                float y[32];
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    float s = i == lane ? 1.0f : 0.0f;
+                for (int i = 0; i < 32; i++) {
+                    float s0 = i == lane ? 1.0f : 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < i; j++) s = fmaf(-a[i * RK_PITCH + j], x[j], s);
-                    x[i] = s;
-                    o[i * RK_PITCH] = s;
+                    for (int j = 0; j < i; j += 4) {
+                        const float4 u = *reinterpret_cast<const float4 *>(a + i * RK_PITCH + j);
+                        s0 = fmaf(u.x, y[j], s0);
+                        if (j + 1 < i) s1 = fmaf(u.y, y[j + 1], s1);
+                        if (j + 2 < i) s2 = fmaf(u.z, y[j + 2], s2);
+                        if (j + 3 < i) s3 = fmaf(u.w, y[j + 3], s3);
+                    }
+                    y[i] = (s0 + s1) + (s2 + s3);
+                    o[i * RK_PITCH] = y[i];
                 }
             }
             bar_sync(BAR_PROD, RK_PROD);
-            // the blocks below, column by column: T_ij = -T_ii sum_{j <= k < i} A_ik T_kj; a warp takes 8 of a block
-            // column's 16 columns (it reads only what it wrote, and the diagonal)
-            const int jb = wid >> 1, half = (wid & 1) * 8;
-            for (int ib = jb + 1; ib < 4; ib++) {
-                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                for (int k = jb; k < ib; k++)
-                    rk_block(d, As + (16 * ib) * RK_PITCH + 16 * k, Ts + (16 * k) * RK_PITCH + 16 * jb + half, lane);
-                float *o = Ts + (16 * ib + (lane >> 1)) * RK_PITCH + 16 * jb + half + (lane & 1) * 4;
-                *reinterpret_cast<float4 *>(o) = make_float4(d[0], d[1], d[2], d[3]);
-                __syncwarp();
-                float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                rk_block(e, Ts + (16 * ib) * RK_PITCH + 16 * ib, Ts + (16 * ib) * RK_PITCH + 16 * jb + half, lane);
-                __syncwarp();
-                *reinterpret_cast<float4 *>(o) = make_float4(-e[0], -e[1], -e[2], -e[3]);
-                __syncwarp();
-            }
-            bar_sync(BAR_PROD, RK_PROD);
-            {   // T as two f16 terms of scaled rows; row tid / 4, columns 16 (tid % 4) ..: zero above the diagonal blocks
-                const int i = tid >> 2, j0 = (tid & 3) * 16;
-                float x[16];
+            {   // as two f16 terms of scaled rows: row tid / 4, eight columns
+                const int i = tid >> 2, j0 = (tid & 3) * 8;
+                float y[8];
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
+                for (int k = 0; k < 2; k++) {
                     const float4 u = *reinterpret_cast<const float4 *>(Ts + i * RK_PITCH + j0 + 4 * k);
-                    const bool in_ = j0 <= (i & ~15);
-                    x[4 * k] = in_ ? u.x : 0.0f;
-                    x[4 * k + 1] = in_ ? u.y : 0.0f;
-                    x[4 * k + 2] = in_ ? u.z : 0.0f;
-                    x[4 * k + 3] = in_ ? u.w : 0.0f;
+                    y[4 * k] = u.x;
+                    y[4 * k + 1] = u.y;
+                    y[4 * k + 2] = u.z;
+                    y[4 * k + 3] = u.w;
                 }
                 float mx = 0.0f;
 #pragma unroll
-                for (int k = 0; k < 16; k++) mx = fmaxf(mx, fabsf(x[k]));
+                for (int k = 0; k < 8; k++) mx = fmaxf(mx, fabsf(y[k]));
                 float inv;
                 const float s = pow2_scale<12>(quad_max(mx), inv);
-                uint32_t hi[8], lo[8];
+                uint32_t hi[4], lo[4];
 #pragma unroll
-                for (int k = 0; k < 8; k++) split_f16(x[2 * k], x[2 * k + 1], s, hi[k], lo[k]);
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const int off = i * 128 + (((j0 / 8 + k) ^ (i & 7)) << 4);
-                    *reinterpret_cast<uint4 *>(sg + RK_TH + off) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
-                    *reinterpret_cast<uint4 *>(sg + RK_TL + off) = make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
-                }
+                for (int k = 0; k < 4; k++) split_f16(y[2 * k], y[2 * k + 1], s, hi[k], lo[k]);
+                const int off = i * 128 + ((((i >> 5) * 4 + (tid & 3)) ^ (i & 7)) << 4);
+                *reinterpret_cast<uint4 *>(sg + RK_TH + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4 *>(sg + RK_TL + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 if ((tid & 3) == 0) cf[CF_T * RK_C + i] = inv;
             }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         bar_arrive(BAR_FULL + st, RK_THREADS);
     }
 }
 
-// A flagged chunk, token by token: S in the chain's registers, everything else from global memory.
+// A flagged chunk, token by token, everything from global memory (S too: held in an array that a call
+// takes, it would live in local memory on the ordinary path as well).
 template <bool DELTA>
-__device__ __noinline__ void rk_serial(const RecParams &p, float (&S)[16][4], int h, int dv, int32_t t0, int32_t t1) {
+__device__ __noinline__ void rk_serial(const RecParams &p, float *S0, int h, int dv, int32_t t0, int32_t t1) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int hk = h / (p.n_head / p.n_head_k);
+    float2 *S = reinterpret_cast<float2 *>(S0 + g * REC_HD + 2 * t), *Sb = reinterpret_cast<float2 *>(S0 + (g + 8) * REC_HD + 2 * t);
     for (int32_t r = t0; r < t1; r++) {
         const __nv_bfloat162 *k = reinterpret_cast<const __nv_bfloat162 *>(static_cast<const __nv_bfloat16 *>(p.k) + (int64_t)r * p.k_stride + hk * REC_HD);
         const __nv_bfloat162 *q = reinterpret_cast<const __nv_bfloat162 *>(static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)r * p.q_stride + hk * REC_HD);
         const __nv_bfloat16 *v = static_cast<const __nv_bfloat16 *>(p.v) + (int64_t)r * p.v_stride + h * REC_HD + dv;
         const float eg = expf(p.g[(int64_t)r * p.n_head + h]);
         float u0 = __bfloat162float(v[g]), u1 = __bfloat162float(v[g + 8]), d0 = 0.0f, d1 = 0.0f, o0 = 0.0f, o1 = 0.0f;
-#pragma unroll
         for (int n = 0; n < 16; n++) {
             const float2 kf = __bfloat1622float2(k[4 * n + t]);
-#pragma unroll
-            for (int e = 0; e < 4; e++) S[n][e] *= eg;
-            d0 += S[n][0] * kf.x + S[n][1] * kf.y;
-            d1 += S[n][2] * kf.x + S[n][3] * kf.y;
+            d0 += S[4 * n].x * eg * kf.x + S[4 * n].y * eg * kf.y;
+            d1 += Sb[4 * n].x * eg * kf.x + Sb[4 * n].y * eg * kf.y;
         }
         if (DELTA) {
             const float b = p.beta[(int64_t)r * p.n_head + h];
             u0 = b * (u0 - quad_sum(d0));
             u1 = b * (u1 - quad_sum(d1));
         }
-#pragma unroll
         for (int n = 0; n < 16; n++) {
             const float2 kf = __bfloat1622float2(k[4 * n + t]), qf = __bfloat1622float2(q[4 * n + t]);
-            S[n][0] = fmaf(u0, kf.x, S[n][0]);
-            S[n][1] = fmaf(u0, kf.y, S[n][1]);
-            S[n][2] = fmaf(u1, kf.x, S[n][2]);
-            S[n][3] = fmaf(u1, kf.y, S[n][3]);
-            o0 += S[n][0] * qf.x + S[n][1] * qf.y;
-            o1 += S[n][2] * qf.x + S[n][3] * qf.y;
+            const float2 a = S[4 * n], b = Sb[4 * n];
+            const float2 x = make_float2(fmaf(u0, kf.x, a.x * eg), fmaf(u0, kf.y, a.y * eg));
+            const float2 y = make_float2(fmaf(u1, kf.x, b.x * eg), fmaf(u1, kf.y, b.y * eg));
+            S[4 * n] = x;
+            Sb[4 * n] = y;
+            o0 += x.x * qf.x + x.y * qf.y;
+            o1 += y.x * qf.x + y.y * qf.y;
         }
         o0 = quad_sum(o0);
         o1 = quad_sum(o1);
@@ -741,12 +730,22 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, int se
     bar_arrive(BAR_EMPTY, RK_THREADS);
     if (n_chunks > 1) bar_arrive(BAR_EMPTY + 1, RK_THREADS);
     float S[16][4];   // rows dv + g and dv + g + 8, keys 8 n + 2 t, + 1
+    auto load_state = [&]() {
 #pragma unroll
-    for (int n = 0; n < 16; n++) {
-        const float2 a = *reinterpret_cast<const float2 *>(S0 + g * REC_HD + 8 * n + 2 * t);
-        const float2 b = *reinterpret_cast<const float2 *>(S0 + (g + 8) * REC_HD + 8 * n + 2 * t);
-        S[n][0] = a.x; S[n][1] = a.y; S[n][2] = b.x; S[n][3] = b.y;
-    }
+        for (int n = 0; n < 16; n++) {
+            const float2 a = *reinterpret_cast<const float2 *>(S0 + g * REC_HD + 8 * n + 2 * t);
+            const float2 b = *reinterpret_cast<const float2 *>(S0 + (g + 8) * REC_HD + 8 * n + 2 * t);
+            S[n][0] = a.x; S[n][1] = a.y; S[n][2] = b.x; S[n][3] = b.y;
+        }
+    };
+    auto store_state = [&]() {
+#pragma unroll
+        for (int n = 0; n < 16; n++) {
+            *reinterpret_cast<float2 *>(S0 + g * REC_HD + 8 * n + 2 * t) = make_float2(S[n][0], S[n][1]);
+            *reinterpret_cast<float2 *>(S0 + (g + 8) * REC_HD + 8 * n + 2 * t) = make_float2(S[n][2], S[n][3]);
+        }
+    };
+    load_state();
     for (int c = 0; c < n_chunks; c++) {
         const int st = c & 1;
         const int32_t t0 = beg + c * RK_C;
@@ -754,22 +753,33 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, int se
         const uint32_t su = smu + st * RK_STAGE;
         const float *cf = reinterpret_cast<const float *>(sg + RK_COEF);
         bar_sync(BAR_FULL + st, RK_THREADS);
-        if (cf[CF_N * RK_C + 1] != 0.0f) {
-            rk_serial<DELTA>(p, S, h, dv, t0, min(end, t0 + RK_C));
+        const uint32_t vrow = su + RK_V + ((m >> 1) * 8 + r) * (RK_ROWS * 2) + (((2 * wid + (m & 1)) ^ r) << 4);
+        uint32_t v[4][4];   // v of 16 tokens each: rows g, g + 8 of tokens 0 .. 7, then of 8 .. 15
+        uint32_t vm = 0;
+#pragma unroll
+        for (int np = 0; np < 4; np++) {
+            ldsm4t(v[np], vrow + np * 16 * (RK_ROWS * 2));
+#pragma unroll
+            for (int k = 0; k < 4; k++) vm = __vmaxu2(vm, v[np][k] & 0x7fff7fffu);
+        }
+        if (__any_sync(0xffffffffu, (vm & 0xffffu) >= 0x7f80u || vm >= 0x7f800000u || cf[CF_N * RK_C + 1] != 0.0f)) {
+            store_state();
+            rk_serial<DELTA>(p, S0, h, dv, t0, min(end, t0 + RK_C));
+            load_state();
             if (c + 2 < n_chunks) bar_arrive(BAR_EMPTY + st, RK_THREADS);
             continue;
         }
         float s0, s1, is0, is1;
         row_scales(S, s0, s1, is0, is1);
-        // X = S K^T, then R; or V
-        float X[8][4];
+        float X[8][4], O[8][4];
 #pragma unroll
-        for (int n = 0; n < 8; n++) X[n][0] = X[n][1] = X[n][2] = X[n][3] = 0.0f;
+        for (int n = 0; n < 8; n++) X[n][0] = X[n][1] = X[n][2] = X[n][3] = O[n][0] = O[n][1] = O[n][2] = O[n][3] = 0.0f;
+        // X = S K^T (delta rule), O = S Q^T (the leading f16 term alone)
         const uint32_t krow = su + ((m >> 1) * 8 + r) * 256;
-        if (DELTA) {
 #pragma unroll
-            for (int kk = 0; kk < 8; kk++) {
-                uint32_t hi[4], lo[4], b[4];
+        for (int kk = 0; kk < 8; kk++) {
+            uint32_t hi[4], lo[4], b[4];
+            if (DELTA) {
                 split_f16(S[2 * kk][0], S[2 * kk][1], s0, hi[0], lo[0]);
                 split_f16(S[2 * kk][2], S[2 * kk][3], s1, hi[1], lo[1]);
                 split_f16(S[2 * kk + 1][0], S[2 * kk + 1][1], s0, hi[2], lo[2]);
@@ -782,87 +792,112 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, int se
                     mma_f16(X[2 * np], lo, b[0], b[1]);
                     mma_f16(X[2 * np + 1], lo, b[2], b[3]);
                 }
+            } else {
+                hi[0] = pack_f16(S[2 * kk][0] * s0, S[2 * kk][1] * s0);
+                hi[1] = pack_f16(S[2 * kk][2] * s1, S[2 * kk][3] * s1);
+                hi[2] = pack_f16(S[2 * kk + 1][0] * s0, S[2 * kk + 1][1] * s0);
+                hi[3] = pack_f16(S[2 * kk + 1][2] * s1, S[2 * kk + 1][3] * s1);
+            }
+#pragma unroll
+            for (int np = 0; np < 4; np++) {
+                ldsm4(b, krow + RK_Q + np * 4096 + (((2 * kk + (m & 1)) ^ r) << 4));
+                mma_f16(O[2 * np], hi, b[0], b[1]);
+                mma_f16(O[2 * np + 1], hi, b[2], b[3]);
             }
         }
-        const uint32_t vrow = su + RK_V + ((m >> 1) * 8 + r) * (RK_ROWS * 2) + (((2 * wid + (m & 1)) ^ r) << 4);
+        // R = beta (v - e^G X), or v
 #pragma unroll
-        for (int np = 0; np < 4; np++) {
-            uint32_t v[4];
-            ldsm4t(v, vrow + np * 16 * (RK_ROWS * 2));
+        for (int n = 0; n < 8; n++) {
+            float2 cx, cv;
+            if (DELTA) {
+                cx = *reinterpret_cast<const float2 *>(cf + CF_X * RK_C + 8 * n + 2 * t);
+                cv = *reinterpret_cast<const float2 *>(cf + CF_V * RK_C + 8 * n + 2 * t);
+            }
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                float *x = &X[2 * np + (k >> 1)][(k & 1) * 2];
-                const float v0 = __uint_as_float(v[k] << 16), v1 = __uint_as_float(v[k] & 0xffff0000u);
-                if (DELTA) {
-                    const float2 cx = *reinterpret_cast<const float2 *>(cf + CF_X * RK_C + 8 * (2 * np + (k >> 1)) + 2 * t);
-                    const float2 cv = *reinterpret_cast<const float2 *>(cf + CF_V * RK_C + 8 * (2 * np + (k >> 1)) + 2 * t);
-                    const float is = k & 1 ? is1 : is0;
-                    x[0] = fmaf(cx.x * is, x[0], cv.x * v0);
-                    x[1] = fmaf(cx.y * is, x[1], cv.y * v1);
-                } else {
-                    x[0] = v0;
-                    x[1] = v1;
-                }
+            for (int k = 0; k < 2; k++) {
+                const uint32_t w = v[n >> 1][(n & 1) * 2 + k];
+                const float v0 = __uint_as_float(w << 16), v1 = __uint_as_float(w & 0xffff0000u), is = k ? is1 : is0;
+                X[n][2 * k] = DELTA ? fmaf(cx.x * is, X[n][2 * k], cv.x * v0) : v0;
+                X[n][2 * k + 1] = DELTA ? fmaf(cx.y * is, X[n][2 * k + 1], cv.y * v1) : v1;
             }
         }
         const uint32_t trow = su + ((m >> 1) * 8 + r) * 128;   // T and P: rows 16 ip + .., chunks 2 jj + ..
-        if (DELTA) {   // U = R T^T
-            float r0, r1, ir0, ir1;
-            row_scales(X, r0, r1, ir0, ir1);
-            uint32_t hi[4][4], lo[4][4];
+        // U = T R by halves of 32 tokens: U_0 = T_0 R_0, R_1 -= A_10 U_0, U_1 = T_1 R_1.  Two f16 terms of both
+        // factors, three products.  X[n] (n = 4 half ..) becomes u times k's scale.
+        if (DELTA) {
 #pragma unroll
-            for (int jj = 0; jj < 4; jj++) {
-                split_f16(X[2 * jj][0], X[2 * jj][1], r0, hi[jj][0], lo[jj][0]);
-                split_f16(X[2 * jj][2], X[2 * jj][3], r1, hi[jj][1], lo[jj][1]);
-                split_f16(X[2 * jj + 1][0], X[2 * jj + 1][1], r0, hi[jj][2], lo[jj][2]);
-                split_f16(X[2 * jj + 1][2], X[2 * jj + 1][3], r1, hi[jj][3], lo[jj][3]);
-            }
+            for (int half = 0; half < 2; half++) {
+                float (&R)[4][4] = *reinterpret_cast<float (*)[4][4]>(&X[4 * half]);
+                float r0, r1, ir0, ir1;
+                uint32_t hi[2][4], lo[2][4];
+                auto split = [&]() {
+                    row_scales(R, r0, r1, ir0, ir1);
 #pragma unroll
-            for (int n = 0; n < 8; n++) X[n][0] = X[n][1] = X[n][2] = X[n][3] = 0.0f;
-#pragma unroll
-            for (int jj = 0; jj < 4; jj++)
-#pragma unroll
-                for (int ip = jj; ip < 4; ip++) {
+                    for (int jj = 0; jj < 2; jj++) {
+                        split_f16(R[2 * jj][0], R[2 * jj][1], r0, hi[jj][0], lo[jj][0]);
+                        split_f16(R[2 * jj][2], R[2 * jj][3], r1, hi[jj][1], lo[jj][1]);
+                        split_f16(R[2 * jj + 1][0], R[2 * jj + 1][1], r0, hi[jj][2], lo[jj][2]);
+                        split_f16(R[2 * jj + 1][2], R[2 * jj + 1][3], r1, hi[jj][3], lo[jj][3]);
+                    }
+                };
+                auto product = [&](float (&d)[2][4], int ip, int jj, int col) {   // tokens 16 ip .., columns 16 col ..
                     uint32_t bh[4], bl[4];
-                    ldsm4(bh, trow + RK_TH + ip * 2048 + (((2 * jj + (m & 1)) ^ r) << 4));
-                    ldsm4(bl, trow + RK_TL + ip * 2048 + (((2 * jj + (m & 1)) ^ r) << 4));
-                    mma_f16(X[2 * ip], hi[jj], bh[0], bh[1]);
-                    mma_f16(X[2 * ip + 1], hi[jj], bh[2], bh[3]);
-                    mma_f16(X[2 * ip], lo[jj], bh[0], bh[1]);
-                    mma_f16(X[2 * ip + 1], lo[jj], bh[2], bh[3]);
-                    mma_f16(X[2 * ip], hi[jj], bl[0], bl[1]);
-                    mma_f16(X[2 * ip + 1], hi[jj], bl[2], bl[3]);
+                    ldsm4(bh, trow + RK_TH + ip * 2048 + (((2 * col + (m & 1)) ^ r) << 4));
+                    ldsm4(bl, trow + RK_TL + ip * 2048 + (((2 * col + (m & 1)) ^ r) << 4));
+                    mma_f16(d[0], hi[jj], bh[0], bh[1]);
+                    mma_f16(d[1], hi[jj], bh[2], bh[3]);
+                    mma_f16(d[0], lo[jj], bh[0], bh[1]);
+                    mma_f16(d[1], lo[jj], bh[2], bh[3]);
+                    mma_f16(d[0], hi[jj], bl[0], bl[1]);
+                    mma_f16(d[1], hi[jj], bl[2], bl[3]);
+                };
+                split();
+                float d[2][2][4] = {};
+                product(d[0], 2 * half, 0, 2 * half);
+                product(d[1], 2 * half + 1, 0, 2 * half);
+                product(d[1], 2 * half + 1, 1, 2 * half + 1);
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    const float2 ct = *reinterpret_cast<const float2 *>(cf + CF_T * RK_C + 8 * (4 * half + n) + 2 * t);
+                    const float2 ck = *reinterpret_cast<const float2 *>(cf + CF_K * RK_C + 8 * (4 * half + n) + 2 * t);
+                    const float (&e)[4] = d[n >> 1][n & 1];
+                    R[n][0] = e[0] * ir0 * ct.x * ck.x;
+                    R[n][1] = e[1] * ir0 * ct.y * ck.y;
+                    R[n][2] = e[2] * ir1 * ct.x * ck.x;
+                    R[n][3] = e[3] * ir1 * ct.y * ck.y;
                 }
+                if (half == 0) {
+                    split();
+                    float f[2][2][4] = {};
+#pragma unroll
+                    for (int ip = 0; ip < 2; ip++)
+#pragma unroll
+                        for (int jj = 0; jj < 2; jj++) product(f[ip], 2 + ip, jj, jj);
+#pragma unroll
+                    for (int n = 0; n < 4; n++) {
+                        const float2 cb = *reinterpret_cast<const float2 *>(cf + CF_B * RK_C + 32 + 8 * n + 2 * t);
+                        const float (&e)[4] = f[n >> 1][n & 1];
+                        X[4 + n][0] = fmaf(cb.x * ir0, e[0], X[4 + n][0]);
+                        X[4 + n][1] = fmaf(cb.y * ir0, e[1], X[4 + n][1]);
+                        X[4 + n][2] = fmaf(cb.x * ir1, e[2], X[4 + n][2]);
+                        X[4 + n][3] = fmaf(cb.y * ir1, e[3], X[4 + n][3]);
+                    }
+                }
+            }
+        } else {
 #pragma unroll
             for (int n = 0; n < 8; n++) {
-                const float2 ct = *reinterpret_cast<const float2 *>(cf + CF_T * RK_C + 8 * n + 2 * t);
-                X[n][0] *= ct.x * ir0;
-                X[n][1] *= ct.y * ir0;
-                X[n][2] *= ct.x * ir1;
-                X[n][3] *= ct.y * ir1;
+                const float2 ck = *reinterpret_cast<const float2 *>(cf + CF_K * RK_C + 8 * n + 2 * t);
+                X[n][0] *= ck.x;
+                X[n][1] *= ck.y;
+                X[n][2] *= ck.x;
+                X[n][3] *= ck.y;
             }
         }
-        // O = S Q^T and P U: leading f16 terms alone
+        // O = scale (e^G O + P U), leading f16 terms
         {
             float u0, u1, iu0, iu1;
             row_scales(X, u0, u1, iu0, iu1);
-            float O[8][4];
-#pragma unroll
-            for (int n = 0; n < 8; n++) O[n][0] = O[n][1] = O[n][2] = O[n][3] = 0.0f;
-#pragma unroll
-            for (int kk = 0; kk < 8; kk++) {
-                uint32_t a[4], b[4];
-                a[0] = pack_f16(S[2 * kk][0] * s0, S[2 * kk][1] * s0);
-                a[1] = pack_f16(S[2 * kk][2] * s1, S[2 * kk][3] * s1);
-                a[2] = pack_f16(S[2 * kk + 1][0] * s0, S[2 * kk + 1][1] * s0);
-                a[3] = pack_f16(S[2 * kk + 1][2] * s1, S[2 * kk + 1][3] * s1);
-#pragma unroll
-                for (int np = 0; np < 4; np++) {
-                    ldsm4(b, krow + RK_Q + np * 4096 + (((2 * kk + (m & 1)) ^ r) << 4));
-                    mma_f16(O[2 * np], a, b[0], b[1]);
-                    mma_f16(O[2 * np + 1], a, b[2], b[3]);
-                }
-            }
             uint32_t ua[4][4];
 #pragma unroll
             for (int jj = 0; jj < 4; jj++) {
@@ -957,11 +992,7 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, int se
         }
         if (c + 2 < n_chunks) bar_arrive(BAR_EMPTY + st, RK_THREADS);
     }
-#pragma unroll
-    for (int n = 0; n < 16; n++) {
-        *reinterpret_cast<float2 *>(S0 + g * REC_HD + 8 * n + 2 * t) = make_float2(S[n][0], S[n][1]);
-        *reinterpret_cast<float2 *>(S0 + (g + 8) * REC_HD + 8 * n + 2 * t) = make_float2(S[n][2], S[n][3]);
-    }
+    store_state();
 }
 
 template <bool DELTA>
@@ -974,8 +1005,13 @@ __global__ void __launch_bounds__(RK_THREADS, 1) k_rec_chunk(const __grid_consta
         return;
     }
     if (beg == end) return;
-    if (threadIdx.x < RK_PROD) rk_produce<DELTA>(p, rk_sm, h, row0, beg, end);
-    else rk_chain<DELTA>(p, rk_sm, seq, h, row0, beg, end);
+    if (threadIdx.x < RK_PROD) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(RK_PROD_REGS));
+        rk_produce<DELTA>(p, rk_sm, h, row0, beg, end);
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(RK_CHAIN_REGS));
+        rk_chain<DELTA>(p, rk_sm, seq, h, row0, beg, end);
+    }
 }
 
 cudaError_t launch_rec_step(const RecParams &p, cudaStream_t st) {
