@@ -347,17 +347,22 @@ __global__ void __launch_bounds__(RT_THREADS) k_rec_serial(const __grid_constant
 //
 // A zero of T or P times a NaN is a NaN, so a chunk with a non-finite input would spread it to earlier
 // tokens; such chunks are flagged by the producers and run token by token from global memory.
-constexpr int RK_C = 64, RK_NW = 4, RK_PROD = 256, RK_THREADS = RK_PROD + RK_NW * 32;
+constexpr int RK_C = 64, RK_NW = 4, RK_GROUPS = 3, RK_GT = 128;    // RK_GROUPS producer groups of RK_GT threads
+constexpr int RK_PROD = RK_GROUPS * RK_GT, RK_THREADS = RK_PROD + RK_NW * 32;
 constexpr int RK_ROWS = RK_NW * 16;
+// a stage (one per group): k, q, P, T (two terms) and v of a chunk, CF_N arrays of RK_C floats, e^(G_C), the flag
 constexpr int RK_K = 0, RK_Q = 16384, RK_P = 32768, RK_TH = 40960, RK_TL = 49152, RK_V = 57344;
-constexpr int RK_COEF = RK_V + RK_C * RK_ROWS * 2;      // CF_N arrays of RK_C floats, then e^(G_C) and the flag
-enum { CF_X, CF_V, CF_T, CF_Q1, CF_Q2, CF_W, CF_K, CF_B, CF_N };
+constexpr int RK_COEF = RK_V + RK_C * RK_ROWS * 2;
+enum { CF_G, CF_V, CF_T, CF_Q, CF_W, CF_K, CF_B, CF_N };
 constexpr int RK_STAGE = RK_COEF + CF_N * RK_C * 4 + 128;
-constexpr int RK_PITCH = 36;                            // floats per row of the 32 x 32 triangular blocks
-constexpr int RK_A = 2 * RK_STAGE, RK_T = RK_A + RK_C * RK_PITCH * 4, RK_SMALL = RK_T + RK_C * RK_PITCH * 4;
-constexpr int RK_SMEM = RK_SMALL + 6 * RK_C * 4;
-constexpr int RK_PROD_REGS = 104, RK_CHAIN_REGS = 240;  // of 168 at launch: 256 x 104 + 128 x 240 <= 384 x 168
-enum { BAR_FULL = 1, BAR_EMPTY = 3, BAR_PROD = 5 };
+// a group's scratch: A, then T, as 16 x 16 tiles (per 32 x 32 block: diagonal, below, diagonal), and per-token values
+constexpr int RK_PITCH = 20, RK_TILE = 16 * RK_PITCH;
+constexpr int RK_SCRATCH = 6 * RK_TILE * 4 + 6 * RK_C * 4;
+constexpr int RK_SMEM = RK_GROUPS * (RK_STAGE + RK_SCRATCH);
+static_assert(RK_SMEM <= 232448, "shared memory of a CTA");
+constexpr int RK_PROD_REGS = 96, RK_CHAIN_REGS = 224;   // of 128 at launch: 384 x 96 + 128 x 224 = 512 x 128
+enum { BAR_FULL = 1, BAR_EMPTY = BAR_FULL + RK_GROUPS, BAR_PROD = BAR_EMPTY + RK_GROUPS };
+constexpr int RK_PAIR = RK_GT + RK_NW * 32;             // threads that meet at a stage's barriers
 
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ void bar_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
@@ -426,23 +431,17 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ void rk_cp16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-// Sixteen words of bf16 pairs, four lanes holding a row of 128: to f16, the row scaled by a power of two to
-// [1, 2).  dst: the row; lane l holds its 16-byte chunks l, l + 4, l + 8, l + 12.  Returns the inverse scale.
-__device__ __forceinline__ float rk_row_f16(const uint4 (&u)[4], uint8_t *dst, int l, int sw, bool &bad) {
-    uint32_t m = 0;
+// Sixteen words of bf16 pairs, four lanes holding a row of 128 (lane l its 16-byte chunks l, l + 4, l + 8, l + 12).
+// Bits of the row's largest magnitude (a NaN is above infinity).
+__device__ __forceinline__ uint32_t rk_row_max(const uint4 (&u)[4]) {
+    uint32_t m[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        m = __vmaxu2(m, u[i].x & 0x7fff7fffu);
-        m = __vmaxu2(m, u[i].y & 0x7fff7fffu);
-        m = __vmaxu2(m, u[i].z & 0x7fff7fffu);
-        m = __vmaxu2(m, u[i].w & 0x7fff7fffu);
-    }
-    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    m = max(m & 0xffffu, m >> 16);           // bits of the largest magnitude; a NaN is above infinity
-    bad |= m >= 0x7f80u;
-    float inv;
-    const float s = pow2_scale<0>(__uint_as_float(m << 16), inv);
+    for (int i = 0; i < 4; i++)
+        m[i] = __vmaxu2(__vmaxu2(u[i].x & 0x7fff7fffu, u[i].y & 0x7fff7fffu), __vmaxu2(u[i].z & 0x7fff7fffu, u[i].w & 0x7fff7fffu));
+    return __vmaxu2(__vmaxu2(m[0], m[1]), __vmaxu2(m[2], m[3]));
+}
+// The row to f16, times a power of two.
+__device__ __forceinline__ void rk_row_f16(const uint4 (&u)[4], float s, uint8_t *dst, int l, int sw) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
@@ -451,63 +450,95 @@ __device__ __forceinline__ float rk_row_f16(const uint4 (&u)[4], uint8_t *dst, i
         for (int j = 0; j < 4; j++) o[j] = pack_f16(__uint_as_float(w[j] << 16) * s, __uint_as_float(w[j] & 0xffff0000u) * s);
         *reinterpret_cast<uint4 *>(dst + (((l + 4 * i) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
     }
-    return inv;
+}
+// The lane's four columns of a 16 x 16 by 16 x 8 product: row a, columns b (pitch RK_PITCH).
+__device__ __forceinline__ float4 rk_block(const float *a, const float *b) {
+    float4 d = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int k4 = 0; k4 < 4; k4++) {
+        const float4 u = *reinterpret_cast<const float4 *>(a + 4 * k4);
+        const float x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float4 y = *reinterpret_cast<const float4 *>(b + (4 * k4 + k) * RK_PITCH);
+            d.x = fmaf(x[k], y.x, d.x);
+            d.y = fmaf(x[k], y.y, d.y);
+            d.z = fmaf(x[k], y.z, d.z);
+            d.w = fmaf(x[k], y.w, d.w);
+        }
+    }
+    return d;
 }
 
+// A producer group: chunks grp, grp + RK_GROUPS, ... of the sequence, each into the group's own stage.
 template <bool DELTA>
 __device__ __forceinline__ void rk_produce(const RecParams &p, uint8_t *sm, int h, int row0, int32_t beg, int32_t end) {
-    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int grp = threadIdx.x / RK_GT, tid = threadIdx.x % RK_GT, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
     const int hk = h / (p.n_head / p.n_head_k);
-    float *As = reinterpret_cast<float *>(sm + RK_A), *Ts = reinterpret_cast<float *>(sm + RK_T);
-    float *gs = reinterpret_cast<float *>(sm + RK_SMALL), *bs = gs + RK_C, *Gh = bs + RK_C, *Gl = Gh + RK_C, *iK = Gl + RK_C,
-          *iQ = iK + RK_C;
-    const uint32_t smu = (uint32_t)__cvta_generic_to_shared(sm);
-    // This thread's row of k and q (a permutation within eight: the two rows of eight lanes differ in bit 2, so
-    // their swizzled 16-byte stores meet different banks) and its rows of v.
+    uint8_t *sg = sm + grp * RK_STAGE;
+    const uint32_t su = (uint32_t)__cvta_generic_to_shared(sg);
+    float *cf = reinterpret_cast<float *>(sg + RK_COEF);
+    float *As = reinterpret_cast<float *>(sm + RK_GROUPS * RK_STAGE + grp * RK_SCRATCH);
+    float *gs = As + 6 * RK_TILE, *bs = gs + RK_C, *iK = bs + RK_C, *iQ = iK + RK_C;
+    float2 *G2 = reinterpret_cast<float2 *>(iQ + RK_C);   // sums of g up to a token, as two floats
+    // This thread's rows of k and q: this one and 32 below (a permutation within eight: the two rows of eight lanes
+    // differ in bit 2, so their swizzled 16-byte stores meet different banks), and of v.
     const int x = tid >> 2, row = (x & ~7) | ((x & 1) << 2) | ((x >> 1) & 3);
-    const __nv_bfloat16 *kp = static_cast<const __nv_bfloat16 *>(p.k) + (int64_t)(beg + row) * p.k_stride + (int64_t)hk * REC_HD + t * 8;
-    const __nv_bfloat16 *qp = static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)(beg + row) * p.q_stride + (int64_t)hk * REC_HD + t * 8;
-    const __nv_bfloat16 *vp = static_cast<const __nv_bfloat16 *>(p.v) + (int64_t)(beg + (tid >> 3)) * p.v_stride + (int64_t)h * REC_HD + row0 + (tid & 7) * 8;
-    uint4 ku[4], qu[4];
-    float gu = 0.0f, bu = 0.0f;
-    auto load = [&](int32_t t0) {
-        const bool ok = t0 + row < end;
+    const int32_t first = beg + grp * RK_C;
+    const __nv_bfloat16 *kp = static_cast<const __nv_bfloat16 *>(p.k) + (int64_t)(first + row) * p.k_stride + (int64_t)hk * REC_HD + t * 8;
+    const __nv_bfloat16 *qp = static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)(first + row) * p.q_stride + (int64_t)hk * REC_HD + t * 8;
+    const __nv_bfloat16 *vp = static_cast<const __nv_bfloat16 *>(p.v) + (int64_t)(first + (tid >> 3)) * p.v_stride + (int64_t)h * REC_HD + row0 + (tid & 7) * 8;
+    // This warp's 16 x 16 tiles of scores, on and below the diagonal: ten of q k^T, then (delta rule) ten of k k^T,
+    // of which six lie in the two 32 x 32 blocks of T (tib / 2 == tjb / 2).
+    constexpr int NT = DELTA ? 20 : 10;
+    const int m = lane >> 3, r = lane & 7;
+    for (int32_t t0 = first; t0 < end; t0 += RK_GROUPS * RK_C) {
+        uint4 ku[2][4], qu[2][4];
+        float gu = 0.0f, bu = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            ku[i] = ok ? *reinterpret_cast<const uint4 *>(kp + 32 * i) : make_uint4(0, 0, 0, 0);
-            qu[i] = ok ? *reinterpret_cast<const uint4 *>(qp + 32 * i) : make_uint4(0, 0, 0, 0);
+        for (int a = 0; a < 2; a++) {
+            const bool ok = t0 + 32 * a + row < end;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                ku[a][i] = ok ? *reinterpret_cast<const uint4 *>(kp + 32 * a * p.k_stride + 32 * i) : make_uint4(0, 0, 0, 0);
+                qu[a][i] = ok ? *reinterpret_cast<const uint4 *>(qp + 32 * a * p.q_stride + 32 * i) : make_uint4(0, 0, 0, 0);
+            }
         }
-        kp += RK_C * p.k_stride;
-        qp += RK_C * p.q_stride;
-        gu = bu = 0.0f;
         if (tid < RK_C && t0 + tid < end) {
             gu = p.g[(int64_t)(t0 + tid) * p.n_head + h];
             if (DELTA) bu = p.beta[(int64_t)(t0 + tid) * p.n_head + h];
         }
-    };
-    load(beg);
-    int c = 0;
-    for (int32_t t0 = beg; t0 < end; t0 += RK_C, c++) {
-        const int st = c & 1;
-        uint8_t *sg = sm + st * RK_STAGE;
-        const uint32_t su = smu + st * RK_STAGE;
-        float *cf = reinterpret_cast<float *>(sg + RK_COEF);
-        bar_sync(BAR_EMPTY + st, RK_THREADS);
+        bar_sync(BAR_EMPTY + grp, RK_PAIR);
 #pragma unroll
-        for (int i = 0; i < 2; i++) {   // v as it is, zeros behind the sequence
-            const int r = 32 * i + (tid >> 3), ch = tid & 7;
-            const uint32_t off = RK_V + r * (RK_ROWS * 2) + ((ch ^ (r & 7)) << 4);
-            if (t0 + r < end) rk_cp16(su + off, vp + 32 * i * p.v_stride);
+        for (int i = 0; i < 4; i++) {   // v as it is, zeros behind the sequence
+            const int vr = 16 * i + (tid >> 3), ch = tid & 7;
+            const uint32_t off = RK_V + vr * (RK_ROWS * 2) + ((ch ^ (vr & 7)) << 4);
+            if (t0 + vr < end) rk_cp16(su + off, vp + 16 * i * p.v_stride);
             else *reinterpret_cast<uint4 *>(sg + off) = make_uint4(0, 0, 0, 0);
         }
-        vp += RK_C * p.v_stride;
+        kp += RK_GROUPS * RK_C * p.k_stride;
+        qp += RK_GROUPS * RK_C * p.q_stride;
+        vp += RK_GROUPS * RK_C * p.v_stride;
         bool bad = false;
         if (tid == 0) cf[CF_N * RK_C + 1] = 0.0f;
-        const float ik = rk_row_f16(ku, sg + RK_K + row * 256, t, row & 7, bad);
-        const float iq = rk_row_f16(qu, sg + RK_Q + row * 256, t, row & 7, bad);
-        if (t == 0) {
-            iK[row] = ik;
-            iQ[row] = iq;
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            uint32_t mk = rk_row_max(ku[a]), mq = rk_row_max(qu[a]);
+            mk = __vmaxu2(mk, __shfl_xor_sync(0xffffffffu, mk, 1));
+            mq = __vmaxu2(mq, __shfl_xor_sync(0xffffffffu, mq, 1));
+            mk = __vmaxu2(mk, __shfl_xor_sync(0xffffffffu, mk, 2));
+            mq = __vmaxu2(mq, __shfl_xor_sync(0xffffffffu, mq, 2));
+            mk = max(mk & 0xffffu, mk >> 16);
+            mq = max(mq & 0xffffu, mq >> 16);
+            bad |= max(mk, mq) >= 0x7f80u;
+            float ik, iq;
+            const float sk = pow2_scale<0>(__uint_as_float(mk << 16), ik), sq = pow2_scale<0>(__uint_as_float(mq << 16), iq);
+            rk_row_f16(ku[a], sk, sg + RK_K + (32 * a + row) * 256, t, row & 7);
+            rk_row_f16(qu[a], sq, sg + RK_Q + (32 * a + row) * 256, t, row & 7);
+            if (t == 0) {
+                iK[32 * a + row] = ik;
+                iQ[32 * a + row] = iq;
+            }
         }
         if (tid < RK_C) {
             // in base 2; below 2^-184 = 0: the clamp keeps sums and differences finite.  A growing state
@@ -516,10 +547,9 @@ __device__ __forceinline__ void rk_produce(const RecParams &p, uint8_t *sm, int 
             bs[tid] = bu;
             bad |= !(gu <= 0.0f) || !(fabsf(bu) <= 3.0e38f);
         }
-        load(t0 + RK_C);
-        bar_sync(BAR_PROD, RK_PROD);
+        bar_sync(BAR_PROD + grp, RK_GT);
         if (bad) cf[CF_N * RK_C + 1] = 1.0f;
-        if (wid == 7) {
+        if (wid == 3) {
             // sums of g as pairs of floats (two-sum at each step), two tokens per lane
             const float g0 = gs[2 * lane], g1 = gs[2 * lane + 1];
             float hi = g0 + g1, lo = (g0 - (hi - (hi - g0))) + (g1 - (hi - g0));
@@ -533,146 +563,191 @@ __device__ __forceinline__ void rk_produce(const RecParams &p, uint8_t *sm, int 
                     lo = e - (hi - s);
                 }
             }
-            Gh[2 * lane + 1] = hi;
-            Gl[2 * lane + 1] = lo;
             const float s = hi - g1, b = s - hi;
-            const float e = (hi - (s - b)) + (-g1 - b) + lo;
-            Gh[2 * lane] = s + e;
-            Gl[2 * lane] = e - ((s + e) - s);
+            const float e = (hi - (s - b)) + (-g1 - b) + lo, f = s + e;
+            *reinterpret_cast<float4 *>(G2 + 2 * lane) = make_float4(f, e - (f - s), hi, lo);
         }
-        // Scores, in 16 x 16 tiles on and below the diagonal: ten of q k^T, then (delta rule) ten of k k^T, spread
-        // over the warps; warp 7 has the sums of g and the fewest.
-        constexpr int NT = DELTA ? 20 : 10, PER = DELTA ? 3 : 2;
-        float acc[PER][2][4];
-        uint32_t arow[PER], brow[PER];
-        const int m = lane >> 3, r = lane & 7;
+        // Two passes over the warp's tiles (ids wid + 4 k), as registers allow.
 #pragma unroll
-        for (int k = 0; k < PER; k++) {
-            const int id = min(wid + 8 * k, NT - 1), tt = id % 10, ib = tt < 1 ? 0 : tt < 3 ? 1 : tt < 6 ? 2 : 3, jb = tt - ib * (ib + 1) / 2;
-            arow[k] = su + (id < 10 ? RK_Q : RK_K) + (16 * ib + (m & 1) * 8 + r) * 256;
-            brow[k] = su + RK_K + (16 * jb + (m >> 1) * 8 + r) * 256;
+        for (int pass = 0; pass < (DELTA ? 2 : 1); pass++) {
+            constexpr int PER = 3;
+            const int k0 = 3 * pass, id0 = wid + 4 * k0;
+            float acc[PER][2][4];
+            uint32_t arow[PER], brow[PER];
+            int tib[PER], tjb[PER];
 #pragma unroll
-            for (int n = 0; n < 2; n++) acc[k][n][0] = acc[k][n][1] = acc[k][n][2] = acc[k][n][3] = 0.0f;
-        }
+            for (int k = 0; k < PER; k++) {
+                const int id = min(id0 + 4 * k, NT - 1), tt = id < 10 ? id : id - 10;
+                tib[k] = tt < 1 ? 0 : tt < 3 ? 1 : tt < 6 ? 2 : 3;
+                tjb[k] = tt - tib[k] * (tib[k] + 1) / 2;
+                arow[k] = su + (id < 10 ? RK_Q : RK_K) + (16 * tib[k] + (m & 1) * 8 + r) * 256;
+                brow[k] = su + RK_K + (16 * tjb[k] + (m >> 1) * 8 + r) * 256;
 #pragma unroll
-        for (int kk = 0; kk < 8; kk++) {
+                for (int n = 0; n < 2; n++) acc[k][n][0] = acc[k][n][1] = acc[k][n][2] = acc[k][n][3] = 0.0f;
+            }
 #pragma unroll
-            for (int k = 0; k < PER; k++)
-                if (8 * k + 8 <= NT || wid + 8 * k < NT) {
-                    uint32_t a[4], b[4];
-                    ldsm4(a, arow[k] + (((2 * kk + (m >> 1)) ^ r) << 4));
-                    ldsm4(b, brow[k] + (((2 * kk + (m & 1)) ^ r) << 4));
-                    mma_f16(acc[k][0], a, b[0], b[1]);
-                    mma_f16(acc[k][1], a, b[2], b[3]);
-                }
-        }
-        bar_sync(BAR_PROD, RK_PROD);
-        if (tid < RK_C) {
-            const float gam = ex2(Gh[tid]) * fmaf(Gl[tid], 0.6931471805599453f, 1.0f);
-            const float end_g = ex2((Gh[RK_C - 1] - Gh[tid]) + (Gl[RK_C - 1] - Gl[tid]));
-            cf[CF_X * RK_C + tid] = -bs[tid] * gam * iK[tid];
-            cf[CF_V * RK_C + tid] = bs[tid];
-            cf[CF_Q1 * RK_C + tid] = p.scale * gam * iQ[tid];
-            cf[CF_Q2 * RK_C + tid] = p.scale * iQ[tid];
-            cf[CF_W * RK_C + tid] = end_g;
-            cf[CF_K * RK_C + tid] = iK[tid];
-            cf[CF_B * RK_C + tid] = -bs[tid] * iK[tid];
-            if (tid == RK_C - 1) cf[CF_N * RK_C] = gam;
-        }
+            for (int kk = 0; kk < 8; kk++) {
+                uint32_t fa[PER][4], fb[PER][4];
 #pragma unroll
-        for (int k = 0; k < PER; k++)
-            if (8 * k + 8 <= NT || wid + 8 * k < NT) {
-                const int id = wid + 8 * k, tt = id % 10, ib = tt < 1 ? 0 : tt < 3 ? 1 : tt < 6 ? 2 : 3, jb = tt - ib * (ib + 1) / 2;
-                const int i0 = 16 * ib + g, i1 = i0 + 8;
-                const float h0 = Gh[i0], l0 = Gl[i0], h1 = Gh[i1], l1 = Gl[i1];
-                const int s0 = i0 & 7;
-#pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    const int j = 16 * jb + 8 * n + 2 * t;
-                    const float2 hj = *reinterpret_cast<const float2 *>(Gh + j), lj = *reinterpret_cast<const float2 *>(Gl + j);
-                    float *a = acc[k][n];
-                    a[0] *= ex2((h0 - hj.x) + (l0 - lj.x));
-                    a[1] *= ex2((h0 - hj.y) + (l0 - lj.y));
-                    a[2] *= ex2((h1 - hj.x) + (l1 - lj.x));
-                    a[3] *= ex2((h1 - hj.y) + (l1 - lj.y));
-                    if (ib == jb) {
-                        a[0] = j <= i0 ? a[0] : 0.0f;
-                        a[1] = j < i0 ? a[1] : 0.0f;
-                        a[2] = j <= i1 ? a[2] : 0.0f;
-                        a[3] = j < i1 ? a[3] : 0.0f;
+                for (int k = 0; k < PER; k++)
+                    if (4 * (k0 + k) + 4 <= NT || id0 + 4 * k < NT) {
+                        ldsm4(fa[k], arow[k] + (((2 * kk + (m >> 1)) ^ r) << 4));
+                        ldsm4(fb[k], brow[k] + (((2 * kk + (m & 1)) ^ r) << 4));
                     }
-                    const int off = i0 * 128 + (((2 * jb + n) ^ s0) << 4) + t * 4;   // row i1: 8 rows below, the same swizzle
-                    if (id < 10) {
-                        *reinterpret_cast<uint32_t *>(sg + RK_P + off) = pack_f16(a[0], a[1]);
-                        *reinterpret_cast<uint32_t *>(sg + RK_P + off + 1024) = pack_f16(a[2], a[3]);
-                    } else if (ib >= 2 && jb < 2) {   // A's lower left 32 x 32 quarter, |.| <= 512 without k's scales and beta
-                        uint32_t hi, lo;
-                        split_f16(a[0], a[1], 1.0f, hi, lo);
-                        *reinterpret_cast<uint32_t *>(sg + RK_TH + off) = hi;
-                        *reinterpret_cast<uint32_t *>(sg + RK_TL + off) = lo;
-                        split_f16(a[2], a[3], 1.0f, hi, lo);
-                        *reinterpret_cast<uint32_t *>(sg + RK_TH + off + 1024) = hi;
-                        *reinterpret_cast<uint32_t *>(sg + RK_TL + off + 1024) = lo;
-                    } else {
-                        const float b0 = -bs[i0] * iK[i0], b1 = -bs[i1] * iK[i1];
-                        const float2 kj = *reinterpret_cast<const float2 *>(iK + j);
-                        float *o = As + i0 * RK_PITCH + (j & 31);
-                        *reinterpret_cast<float2 *>(o) = make_float2(a[0] * b0 * kj.x, a[1] * b0 * kj.y);
-                        *reinterpret_cast<float2 *>(o + 8 * RK_PITCH) = make_float2(a[2] * b1 * kj.x, a[3] * b1 * kj.y);
+#pragma unroll
+                for (int k = 0; k < PER; k++)
+                    if (4 * (k0 + k) + 4 <= NT || id0 + 4 * k < NT) {
+                        mma_f16(acc[k][0], fa[k], fb[k][0], fb[k][1]);
+                        mma_f16(acc[k][1], fa[k], fb[k][2], fb[k][3]);
                     }
+            }
+            if (pass == 0) {
+                bar_sync(BAR_PROD + grp, RK_GT);
+                if (tid < RK_C) {
+                    const float2 mine = G2[tid], last = G2[RK_C - 1];
+                    const float mik = iK[tid], miq = iQ[tid], mb = bs[tid];
+                    const float gam = ex2(mine.x) * fmaf(mine.y, 0.6931471805599453f, 1.0f);
+                    cf[CF_G * RK_C + tid] = gam;
+                    cf[CF_V * RK_C + tid] = mb;
+                    cf[CF_Q * RK_C + tid] = p.scale * miq;
+                    cf[CF_W * RK_C + tid] = ex2((last.x - mine.x) + (last.y - mine.y));
+                    cf[CF_K * RK_C + tid] = mik;
+                    cf[CF_B * RK_C + tid] = -mb * mik;
+                    if (tid == RK_C - 1) cf[CF_N * RK_C] = gam;
                 }
             }
-        if (DELTA) {
-            bar_sync(BAR_PROD, RK_PROD);
-            // T's two diagonal 32 x 32 blocks by forward substitution, one warp each, a column per lane:
-            // x_i = [i = column] - sum_{j < i} A_ij x_j   (As holds -A)
-            if (wid < 2) {
-                const float *a = As + 32 * wid * RK_PITCH;
-                float *o = Ts + 32 * wid * RK_PITCH + lane;
-                float y[32];
+            // times e^(G_i - G_j); everything is read before anything is written
+            float4 cg[PER][2];
+            float2 rg[PER][2];
 #pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    float s0 = i == lane ? 1.0f : 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
+            for (int k = 0; k < PER; k++) {
+                rg[k][0] = G2[16 * tib[k] + g];
+                rg[k][1] = G2[16 * tib[k] + g + 8];
+#pragma unroll
+                for (int n = 0; n < 2; n++) cg[k][n] = *reinterpret_cast<const float4 *>(G2 + 16 * tjb[k] + 8 * n + 2 * t);
+            }
+            float kb[PER][2];
+            float2 kj[PER][2];
+#pragma unroll
+            for (int k = 0; k < PER; k++)
+                if (k0 + k >= 2) {   // tiles of k k^T begin with the third
+                    kb[k][0] = -bs[16 * tib[k] + g] * iK[16 * tib[k] + g];
+                    kb[k][1] = -bs[16 * tib[k] + g + 8] * iK[16 * tib[k] + g + 8];
+#pragma unroll
+                    for (int n = 0; n < 2; n++) kj[k][n] = *reinterpret_cast<const float2 *>(iK + 16 * tjb[k] + 8 * n + 2 * t);
+                }
+#pragma unroll
+            for (int k = 0; k < PER; k++)
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    float *a = acc[k][n];
+                    a[0] *= ex2((rg[k][0].x - cg[k][n].x) + (rg[k][0].y - cg[k][n].y));
+                    a[1] *= ex2((rg[k][0].x - cg[k][n].z) + (rg[k][0].y - cg[k][n].w));
+                    a[2] *= ex2((rg[k][1].x - cg[k][n].x) + (rg[k][1].y - cg[k][n].y));
+                    a[3] *= ex2((rg[k][1].x - cg[k][n].z) + (rg[k][1].y - cg[k][n].w));
+                    if (tib[k] == tjb[k]) {
+                        const int j = 8 * n + 2 * t;
+                        a[0] = j <= g ? a[0] : 0.0f;
+                        a[1] = j < g ? a[1] : 0.0f;
+                        a[2] = j <= g + 8 ? a[2] : 0.0f;
+                        a[3] = j < g + 8 ? a[3] : 0.0f;
+                    }
+                }
+#pragma unroll
+            for (int k = 0; k < PER; k++)
+                if (4 * (k0 + k) + 4 <= NT || id0 + 4 * k < NT) {
+                    const int i0 = 16 * tib[k] + g;
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        const float *a = acc[k][n];
+                        const int off = i0 * 128 + (((2 * tjb[k] + n) ^ (g & 7)) << 4) + t * 4;   // row i0 + 8: the same swizzle
+                        if (4 * (k0 + k) + 4 <= 10 || id0 + 4 * k < 10) {
+                            *reinterpret_cast<uint32_t *>(sg + RK_P + off) = pack_f16(a[0], a[1]);
+                            *reinterpret_cast<uint32_t *>(sg + RK_P + off + 1024) = pack_f16(a[2], a[3]);
+                        } else if (tib[k] >= 2 && tjb[k] < 2) {   // A's lower left quarter, |.| <= 512 without k's scales and beta
+                            uint32_t hi, lo;
+                            split_f16(a[0], a[1], 1.0f, hi, lo);
+                            *reinterpret_cast<uint32_t *>(sg + RK_TH + off) = hi;
+                            *reinterpret_cast<uint32_t *>(sg + RK_TL + off) = lo;
+                            split_f16(a[2], a[3], 1.0f, hi, lo);
+                            *reinterpret_cast<uint32_t *>(sg + RK_TH + off + 1024) = hi;
+                            *reinterpret_cast<uint32_t *>(sg + RK_TL + off + 1024) = lo;
+                        } else {   // -A, tile 3 block + 0, 1, 2
+                            float *o = As + ((tib[k] >> 1) * 3 + (tib[k] & 1) + (tjb[k] & 1)) * RK_TILE + g * RK_PITCH + 8 * n + 2 * t;
+                            *reinterpret_cast<float2 *>(o) = make_float2(a[0] * kb[k][0] * kj[k][n].x, a[1] * kb[k][0] * kj[k][n].y);
+                            *reinterpret_cast<float2 *>(o + 8 * RK_PITCH) = make_float2(a[2] * kb[k][1] * kj[k][n].x, a[3] * kb[k][1] * kj[k][n].y);
+                        }
+                    }
+                }
+        }
+        if (DELTA) {
+            bar_sync(BAR_PROD + grp, RK_GT);
+            // T's two diagonal 32 x 32 blocks, in place of A.  The four 16 x 16 blocks on the diagonal by forward
+            // substitution, x_i = [i = column] - sum_{j < i} A_ij x_j, one per warp, a column per lane;
+            if (lane < 16) {
+                float *a = As + ((wid >> 1) * 3 + (wid & 1) * 2) * RK_TILE;
+                float y[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float s0 = i == lane ? 1.0f : 0.0f, s1 = 0.0f;
 #pragma unroll
                     for (int j = 0; j < i; j += 4) {
                         const float4 u = *reinterpret_cast<const float4 *>(a + i * RK_PITCH + j);
                         s0 = fmaf(u.x, y[j], s0);
                         if (j + 1 < i) s1 = fmaf(u.y, y[j + 1], s1);
-                        if (j + 2 < i) s2 = fmaf(u.z, y[j + 2], s2);
-                        if (j + 3 < i) s3 = fmaf(u.w, y[j + 3], s3);
+                        if (j + 2 < i) s0 = fmaf(u.z, y[j + 2], s0);
+                        if (j + 3 < i) s1 = fmaf(u.w, y[j + 3], s1);
                     }
-                    y[i] = (s0 + s1) + (s2 + s3);
-                    o[i * RK_PITCH] = y[i];
+                    y[i] = s0 + s1;
                 }
+                __syncwarp(0xffffu);
+#pragma unroll
+                for (int i = 0; i < 16; i++) a[i * RK_PITCH + lane] = y[i];
             }
-            bar_sync(BAR_PROD, RK_PROD);
-            {   // as two f16 terms of scaled rows: row tid / 4, eight columns
-                const int i = tid >> 2, j0 = (tid & 3) * 8;
-                float y[8];
+            bar_sync(BAR_PROD + grp, RK_GT);
+            {   // then T_10 = -T_11 A_10 T_00, eight columns per warp
+                float *tb = As + (wid >> 1) * 3 * RK_TILE, *o = tb + RK_TILE;
+                const int i = lane >> 1, col = (wid & 1) * 8 + (lane & 1) * 4;
+                const float4 u = rk_block(o + i * RK_PITCH, tb + col);
+                bar_sync(BAR_PROD + grp, RK_GT);
+                *reinterpret_cast<float4 *>(o + i * RK_PITCH + col) = u;
+                __syncwarp();
+                const float4 w = rk_block(tb + 2 * RK_TILE + i * RK_PITCH, o + col);
+                __syncwarp();
+                *reinterpret_cast<float4 *>(o + i * RK_PITCH + col) = w;
+            }
+            bar_sync(BAR_PROD + grp, RK_GT);
+            {   // as two f16 terms of scaled rows: row tid / 2, sixteen columns (none right of the diagonal blocks)
+                const int i = tid >> 1, half = tid & 1;
+                const bool low = i & 16, in_ = low || !half;
+                const float *a = As + ((i >> 5) * 3 + (low ? 1 + half : 0)) * RK_TILE + (i & 15) * RK_PITCH;
+                float y[16], mx = 0.0f;
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const float4 u = *reinterpret_cast<const float4 *>(Ts + i * RK_PITCH + j0 + 4 * k);
-                    y[4 * k] = u.x;
-                    y[4 * k + 1] = u.y;
-                    y[4 * k + 2] = u.z;
-                    y[4 * k + 3] = u.w;
+                for (int k = 0; k < 4; k++) {
+                    const float4 u = *reinterpret_cast<const float4 *>(a + 4 * k);
+                    y[4 * k] = u.x; y[4 * k + 1] = u.y; y[4 * k + 2] = u.z; y[4 * k + 3] = u.w;
                 }
-                float mx = 0.0f;
 #pragma unroll
-                for (int k = 0; k < 8; k++) mx = fmaxf(mx, fabsf(y[k]));
+                for (int k = 0; k < 16; k++) mx = fmaxf(mx, fabsf(y[k]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 float inv;
-                const float s = pow2_scale<12>(quad_max(mx), inv);
-                uint32_t hi[4], lo[4];
+                const float s = pow2_scale<12>(mx, inv);
+                if (in_) {
 #pragma unroll
-                for (int k = 0; k < 4; k++) split_f16(y[2 * k], y[2 * k + 1], s, hi[k], lo[k]);
-                const int off = i * 128 + ((((i >> 5) * 4 + (tid & 3)) ^ (i & 7)) << 4);
-                *reinterpret_cast<uint4 *>(sg + RK_TH + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4 *>(sg + RK_TL + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                if ((tid & 3) == 0) cf[CF_T * RK_C + i] = inv;
+                    for (int c8 = 0; c8 < 2; c8++) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) split_f16(y[8 * c8 + 2 * k], y[8 * c8 + 2 * k + 1], s, hi[k], lo[k]);
+                        const int off = i * 128 + ((((i >> 5) * 4 + half * 2 + c8) ^ (i & 7)) << 4);
+                        *reinterpret_cast<uint4 *>(sg + RK_TH + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4 *>(sg + RK_TL + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                }
+                if (!half) cf[CF_T * RK_C + i] = inv;
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-        bar_arrive(BAR_FULL + st, RK_THREADS);
+        bar_arrive(BAR_FULL + grp, RK_PAIR);
     }
 }
 
@@ -727,8 +802,7 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, int se
     const int dv = row0 + 16 * wid;
     float *S0 = reinterpret_cast<float *>(p.state + (int64_t)p.slot[seq] * p.slot_bytes) + ((int64_t)h * REC_HD + dv) * REC_HD;
     const int n_chunks = (end - beg + RK_C - 1) / RK_C;
-    bar_arrive(BAR_EMPTY, RK_THREADS);
-    if (n_chunks > 1) bar_arrive(BAR_EMPTY + 1, RK_THREADS);
+    for (int c = 0; c < min(n_chunks, RK_GROUPS); c++) bar_arrive(BAR_EMPTY + c, RK_PAIR);
     float S[16][4];   // rows dv + g and dv + g + 8, keys 8 n + 2 t, + 1
     auto load_state = [&]() {
 #pragma unroll
@@ -746,13 +820,12 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, int se
         }
     };
     load_state();
-    for (int c = 0; c < n_chunks; c++) {
-        const int st = c & 1;
+    for (int c = 0, st = 0; c < n_chunks; c++, st = st == RK_GROUPS - 1 ? 0 : st + 1) {
         const int32_t t0 = beg + c * RK_C;
         uint8_t *sg = sm + st * RK_STAGE;
         const uint32_t su = smu + st * RK_STAGE;
         const float *cf = reinterpret_cast<const float *>(sg + RK_COEF);
-        bar_sync(BAR_FULL + st, RK_THREADS);
+        bar_sync(BAR_FULL + st, RK_PAIR);
         const uint32_t vrow = su + RK_V + ((m >> 1) * 8 + r) * (RK_ROWS * 2) + (((2 * wid + (m & 1)) ^ r) << 4);
         uint32_t v[4][4];   // v of 16 tokens each: rows g, g + 8 of tokens 0 .. 7, then of 8 .. 15
         uint32_t vm = 0;
@@ -766,7 +839,7 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, int se
             store_state();
             rk_serial<DELTA>(p, S0, h, dv, t0, min(end, t0 + RK_C));
             load_state();
-            if (c + 2 < n_chunks) bar_arrive(BAR_EMPTY + st, RK_THREADS);
+            if (c + RK_GROUPS < n_chunks) bar_arrive(BAR_EMPTY + st, RK_PAIR);
             continue;
         }
         float s0, s1, is0, is1;
@@ -810,7 +883,9 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, int se
         for (int n = 0; n < 8; n++) {
             float2 cx, cv;
             if (DELTA) {
-                cx = *reinterpret_cast<const float2 *>(cf + CF_X * RK_C + 8 * n + 2 * t);
+                const float2 cg = *reinterpret_cast<const float2 *>(cf + CF_G * RK_C + 8 * n + 2 * t);
+                const float2 cb = *reinterpret_cast<const float2 *>(cf + CF_B * RK_C + 8 * n + 2 * t);
+                cx = make_float2(cg.x * cb.x, cg.y * cb.y);
                 cv = *reinterpret_cast<const float2 *>(cf + CF_V * RK_C + 8 * n + 2 * t);
             }
 #pragma unroll
@@ -920,8 +995,9 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, int se
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
                     const int n = 2 * ip + k;
-                    const float2 q1 = *reinterpret_cast<const float2 *>(cf + CF_Q1 * RK_C + 8 * n + 2 * t);
-                    const float2 q2 = *reinterpret_cast<const float2 *>(cf + CF_Q2 * RK_C + 8 * n + 2 * t);
+                    const float2 cg = *reinterpret_cast<const float2 *>(cf + CF_G * RK_C + 8 * n + 2 * t);
+                    const float2 q2 = *reinterpret_cast<const float2 *>(cf + CF_Q * RK_C + 8 * n + 2 * t);
+                    const float2 q1 = make_float2(cg.x * q2.x, cg.y * q2.y);
                     const __nv_bfloat162 a = __floats2bfloat162_rn(fmaf(q1.x * is0, O[n][0], q2.x * iu0 * d[k][0]),
                                                                    fmaf(q1.y * is0, O[n][1], q2.y * iu0 * d[k][1]));
                     const __nv_bfloat162 b = __floats2bfloat162_rn(fmaf(q1.x * is1, O[n][2], q2.x * iu1 * d[k][2]),
@@ -990,7 +1066,7 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, int se
                 }
             }
         }
-        if (c + 2 < n_chunks) bar_arrive(BAR_EMPTY + st, RK_THREADS);
+        if (c + RK_GROUPS < n_chunks) bar_arrive(BAR_EMPTY + st, RK_PAIR);
     }
     store_state();
 }
