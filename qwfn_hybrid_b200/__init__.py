@@ -9,8 +9,8 @@ missing or fails to load, importing the engine raises.
 """
 from __future__ import annotations
 
+import array
 import ctypes
-import math
 import os
 from dataclasses import dataclass, field
 
@@ -150,8 +150,11 @@ def lib() -> ctypes.CDLL:
 
 
 def _i32_array(values) -> ctypes.Array:
-    vals = [int(v) for v in values]
-    return (ctypes.c_int32 * max(1, len(vals)))(*vals)
+    n = len(values)
+    try:   # a few times cheaper than a ctypes constructor per value
+        return (ctypes.c_int32 * n).from_buffer(array.array("i", values)) if n else (ctypes.c_int32 * 1)()
+    except (TypeError, OverflowError):
+        return (ctypes.c_int32 * max(1, n))(*[int(v) for v in values])
 
 
 def _ptr(x) -> int | None:
@@ -166,15 +169,16 @@ def _ptr(x) -> int | None:
 
 
 def _rows(x, dtype: str):
-    """Pointer and row stride (elements) of a tensor of rows [n, ...] whose rows are contiguous."""
+    """Pointer, row stride (elements) and row width of a tensor of rows [n, ...] whose rows are contiguous."""
     if str(x.dtype) != dtype:
         raise ValueError(f"rows of {dtype} wanted, got {x.dtype}")
+    shape, strides = x.shape, x.stride()
     want = 1
-    for d in range(x.dim() - 1, 0, -1):
-        if x.shape[d] > 1 and x.stride(d) != want:
+    for d in range(len(shape) - 1, 0, -1):
+        if shape[d] > 1 and strides[d] != want:
             raise ValueError("each row must be contiguous")
-        want *= x.shape[d]
-    return x.data_ptr(), x.stride(0) if x.shape[0] > 1 else max(x.stride(0), want)
+        want *= shape[d]
+    return x.data_ptr(), strides[0] if shape[0] > 1 else max(strides[0], want), want
 
 
 def _dense(x, dtype: str, n: int, what: str):
@@ -509,7 +513,7 @@ class Engine:
         if kind not in ("torch.float32", "torch.bfloat16") or x.dim() != 2 or x.shape[1] != self.cfg.conv_channels:
             raise ValueError(f"x: F32 or bf16 [n, {self.cfg.conv_channels}] wanted, got {x.dtype} {tuple(x.shape)}")
         n = int(x.shape[0])
-        ptr, stride = _rows(x, kind)
+        ptr, stride, _ = _rows(x, kind)
         self._check(lib().qkv_rec_conv(
             self.handle, rec_layer, _i32_array(slots), _dense(cu, "torch.int32", len(slots) + 1, "cu"), len(slots),
             F32 if kind == "torch.float32" else BF16, ptr, stride,
@@ -518,10 +522,9 @@ class Engine:
 
     def _rec_rows(self, q, k, v, g, beta, n: int, dtype: str) -> QkvRecRows:
         H, hd = self.cfg.rec_n_head, self.cfg.rec_head_dim
-        width, wk, wv = (math.prod(t.shape[1:]) for t in (q, k, v))
-        if any(int(t.shape[0]) != n for t in (q, k, v)) or width % hd or wk != width or wv != H * hd:
+        (qp, qs, width), (kp, ks, wk), (vp, vs, wv) = _rows(q, dtype), _rows(k, dtype), _rows(v, dtype)
+        if not q.shape[0] == k.shape[0] == v.shape[0] == n or width % hd or wk != width or wv != H * hd:
             raise ValueError(f"{n} rows of q and k [heads * {hd}] and v [{H} * {hd}] wanted: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-        (qp, qs), (kp, ks), (vp, vs) = (_rows(t, dtype) for t in (q, k, v))
         return QkvRecRows(qp, kp, vp, qs, ks, vs, _dense(g, "torch.float32", n * H, "g"),
                           _dense(beta, "torch.float32", n * H, "beta"), width // hd)
 

@@ -1,6 +1,6 @@
 // qkv_recurrent.cu -- the recurrent layers' kernels over the engine's state slabs: the short causal
 // convolution (k_rec_conv) and linear attention with a decay per head, with or without the delta rule
-// (k_rec_step for a few tokens, k_rec_serial for prompts).
+// (k_rec_step for a few tokens, k_rec_chunk for prompts).
 #include "qkv_internal.h"
 
 #include <algorithm>
@@ -36,18 +36,18 @@ __device__ __forceinline__ int rec_find(const int32_t *__restrict__ cu, int n_se
 template <typename T> struct RecVec;
 template <> struct RecVec<float> {
     static constexpr int N = 4;
-    static __device__ __forceinline__ void load(const float *p, float (&v)[4]) {
-        const float4 u = *reinterpret_cast<const float4 *>(p);
-        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+    static __device__ __forceinline__ void unpack(const uint4 &u, float (&v)[4]) {
+        v[0] = __uint_as_float(u.x); v[1] = __uint_as_float(u.y); v[2] = __uint_as_float(u.z); v[3] = __uint_as_float(u.w);
     }
+    static __device__ __forceinline__ void load(const float *p, float (&v)[4]) { unpack(*reinterpret_cast<const uint4 *>(p), v); }
     static __device__ __forceinline__ void store(float *p, const float (&v)[4]) {
         *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
     }
 };
 template <> struct RecVec<__nv_bfloat16> {
     static constexpr int N = 8;
-    static __device__ __forceinline__ void load(const __nv_bfloat16 *p, float (&v)[8]) {
-        const uint4 u = *reinterpret_cast<const uint4 *>(p);
+    static __device__ __forceinline__ void load(const __nv_bfloat16 *p, float (&v)[8]) { unpack(*reinterpret_cast<const uint4 *>(p), v); }
+    static __device__ __forceinline__ void unpack(const uint4 &u, float (&v)[8]) {
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -71,14 +71,14 @@ constexpr int RC_THREADS = 256, RC_HIST = 3;
 // The history after the sequence's rows [beg, end) for VEC channels: hist_out[c][j] = row end - 3 + j,
 // of the old history where that lies before beg.
 template <typename T, int VEC>
-__device__ __forceinline__ void rec_conv_hist(const RecConvParams &p, const T *x, int c0, int32_t beg, int32_t end,
+__device__ __forceinline__ void rec_conv_hist(const RecConvParams &p, const T *x, int32_t beg, int32_t end,
                                               const float (&old)[RC_HIST][VEC], float *out) {
     float v[RC_HIST][VEC];
 #pragma unroll
     for (int j = 0; j < RC_HIST; j++) {
         const int32_t r = end - RC_HIST + j;
         if (r >= beg) {
-            RecVec<T>::load(x + (int64_t)r * p.x_stride + c0, v[j]);
+            RecVec<T>::load(x + (int64_t)r * p.x_stride, v[j]);
         } else {
             const int32_t k = r - beg + RC_HIST;   // 0 .. 2: old history
 #pragma unroll
@@ -95,16 +95,30 @@ __device__ __forceinline__ void rec_conv_hist(const RecConvParams &p, const T *x
         reinterpret_cast<float4 *>(out)[i] = make_float4(flat[4 * i], flat[4 * i + 1], flat[4 * i + 2], flat[4 * i + 3]);
 }
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+constexpr int RC_AHEAD = 4;   // rows whose loads are in flight ahead of the ones computed
+
 template <typename T>
-__global__ void __launch_bounds__(RC_THREADS) k_rec_conv(const __grid_constant__ RecConvParams p) {
+__global__ void __launch_bounds__(RC_THREADS, 2) k_rec_conv(const __grid_constant__ RecConvParams p) {
     constexpr int VEC = RecVec<T>::N, LANES = 128 / VEC;
     const int per_row = p.channels / VEC;   // a multiple of LANES
     const int64_t id = (int64_t)blockIdx.x * RC_THREADS + threadIdx.x;
     const int64_t blk = id / per_row;
     const int c0 = (int)(id % per_row) * VEC;
     const int32_t r_lo = (int32_t)min((int64_t)p.n_rows, blk * p.rows_per), r_hi = min(p.n_rows, r_lo + p.rows_per);
-    const T *x = static_cast<const T *>(p.x);
-    T *y = static_cast<T *>(p.y);
+    if (r_lo >= r_hi) return;
+    const T *x = static_cast<const T *>(p.x) + c0;
+    T *y = static_cast<T *>(p.y) + c0;
     float w[VEC][4];
 #pragma unroll
     for (int e = 0; e < VEC; e++) {
@@ -112,16 +126,17 @@ __global__ void __launch_bounds__(RC_THREADS) k_rec_conv(const __grid_constant__
         w[e][0] = u.x; w[e][1] = u.y; w[e][2] = u.z; w[e][3] = u.w;
     }
     const bool norm = c0 < p.n_norm;
+    const float max_inv = 1.0f / p.eps;
     const unsigned lanes = LANES == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
-    float h[RC_HIST][VEC];
-    int32_t beg = 0, end = 0;   // rows of the current sequence
-    for (int32_t r = r_lo; r < r_hi; r++) {
-        if (r >= end || r == r_lo) {
-            const int i = rec_find(p.cu, p.n_seq, p.n_rows, r, beg, end);
-            if (i < 0) {          // a row of no sequence (of this launch)
-                end = 0;
-                continue;
-            }
+    for (int32_t r = r_lo; r < r_hi;) {
+        int32_t beg, end;   // rows of the sequence
+        const int i = rec_find(p.cu, p.n_seq, p.n_rows, r, beg, end);
+        if (i < 0) {        // a row of no sequence (of this launch)
+            r++;
+            continue;
+        }
+        float h[RC_HIST + 1][VEC];   // rows r - 3 .. r
+        {
             float *state = reinterpret_cast<float *>(p.state + (int64_t)p.slot[i] * p.slot_bytes) + (int64_t)c0 * RC_HIST;
             float old[RC_HIST][VEC];
             if (r - beg < RC_HIST) {
@@ -140,7 +155,7 @@ __global__ void __launch_bounds__(RC_THREADS) k_rec_conv(const __grid_constant__
             for (int j = 0; j < RC_HIST; j++) {
                 const int32_t q = r - RC_HIST + j;
                 if (q >= beg) {
-                    RecVec<T>::load(x + (int64_t)q * p.x_stride + c0, h[j]);
+                    RecVec<T>::load(x + (int64_t)q * p.x_stride, h[j]);
                 } else {
                     const int32_t k = q - beg + RC_HIST;
 #pragma unroll
@@ -149,35 +164,50 @@ __global__ void __launch_bounds__(RC_THREADS) k_rec_conv(const __grid_constant__
             }
             if (r == beg) {
                 for (int s = 1; s <= min(p.n_save, end - beg); s++)
-                    rec_conv_hist<T, VEC>(p, x, c0, beg, end - s, old,
+                    rec_conv_hist<T, VEC>(p, x, beg, end - s, old,
                                           reinterpret_cast<float *>(p.back + ((int64_t)p.slot[i] * p.n_rollback + s - 1) * p.slot_bytes) +
                                               (int64_t)c0 * RC_HIST);
-                rec_conv_hist<T, VEC>(p, x, c0, beg, end, old, state);
+                rec_conv_hist<T, VEC>(p, x, beg, end, old, state);
             }
         }
-        float v[VEC], o[VEC];
-        RecVec<T>::load(x + (int64_t)r * p.x_stride + c0, v);
-        float ss = 0.0f;
+        const int32_t lim = min(end, r_hi);
+        const T *xr = x + (int64_t)r * p.x_stride;
+        T *yr = y + (int64_t)r * p.channels;
+        uint4 next[RC_AHEAD];
 #pragma unroll
-        for (int e = 0; e < VEC; e++) {
-            float a = v[e] * w[e][3];
-            a = fmaf(h[0][e], w[e][0], a);
-            a = fmaf(h[1][e], w[e][1], a);
-            a = fmaf(h[2][e], w[e][2], a);
-            o[e] = a / (1.0f + expf(-a));
-            ss = fmaf(o[e], o[e], ss);
-            h[0][e] = h[1][e];
-            h[1][e] = h[2][e];
-            h[2][e] = v[e];
+        for (int k = 0; k < RC_AHEAD; k++)
+            if (r + k < lim) next[k] = *reinterpret_cast<const uint4 *>(xr + k * p.x_stride);
+        for (; r < lim; r += RC_AHEAD) {
+            xr += RC_AHEAD * p.x_stride;
+#pragma unroll
+            for (int k = 0; k < RC_AHEAD; k++) {
+                if (r + k >= lim) break;
+                float (&h0)[VEC] = h[k & 3], (&h1)[VEC] = h[(k + 1) & 3], (&h2)[VEC] = h[(k + 2) & 3], (&v)[VEC] = h[(k + 3) & 3];
+                RecVec<T>::unpack(next[k], v);
+                if (r + RC_AHEAD + k < lim) next[k] = *reinterpret_cast<const uint4 *>(xr + k * p.x_stride);
+                float o[VEC], ss = 0.0f;
+#pragma unroll
+                for (int e = 0; e < VEC; e++) {
+                    float a = v[e] * w[e][3];
+                    a = fmaf(h0[e], w[e][0], a);
+                    a = fmaf(h1[e], w[e][1], a);
+                    a = fmaf(h2[e], w[e][2], a);
+                    o[e] = a * rcp(1.0f + ex2(a * -1.4426950408889634f));
+                    ss = fmaf(o[e], o[e], ss);
+                }
+                if (norm) {   // the lanes of a head walk the same rows: all of them are here
+#pragma unroll
+                    for (int m = LANES / 2; m; m >>= 1) ss += __shfl_xor_sync(lanes, ss, m);
+                    float inv = rsqrtf(ss);
+                    if (inv > max_inv) inv = max_inv;   // (a NaN stays)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) o[e] *= inv;
+                }
+                RecVec<T>::store(yr, o);
+                yr += p.channels;
+            }
         }
-        if (norm) {   // the lanes of a head walk the same rows: all of them are here
-#pragma unroll
-            for (int m = LANES / 2; m; m >>= 1) ss += __shfl_xor_sync(lanes, ss, m);
-            const float inv = 1.0f / fmaxf(sqrtf(ss), p.eps);
-#pragma unroll
-            for (int e = 0; e < VEC; e++) o[e] *= inv;
-        }
-        RecVec<T>::store(y + (int64_t)r * p.channels + c0, o);
+        r = lim;
     }
 }
 
@@ -198,127 +228,107 @@ cudaError_t launch_rec_conv(RecConvParams &p, bool bf16, int num_sms, cudaStream
 // ---------------------------------------------------------------------------- linear attention
 // Per value head with state S [value][key] (key fastest), token by token:
 //   S <- e^g S;  u = v, or with the delta rule u = beta (v - S k);  S <- S + u k^T;  o = scale S q.
-// A value row of S needs no other row, so rows are split over CTAs, warps and lanes freely: 8 lanes
-// per row, each 16 of its 128 keys as four float4 eight apart (a warp's load covers 4 rows in whole
-// 128-byte lines), the row's two dot products by three shuffles.
-constexpr int RT_THREADS = 128, RT_ROWS = 32, RT_TOK = 16;
-constexpr int RT_PASS = RT_ROWS / 16;   // row quads per warp: 4 warps x 4 rows x RT_PASS
+// Bound by the state, read and written once whatever T is.  A value row of S needs no other row: 8 lanes hold
+// a row, each 16 of its 128 keys as four float4 eight apart (a warp's load covers 4 rows in whole 128-byte
+// lines), the row's two dot products are three shuffles, and nothing is shared between warps: every load
+// of a thread -- its part of S and of the T rows of k, q, v -- is issued before the first use.
+constexpr int RT_THREADS = 128, RT_PASS = 2, RT_ROWS = RT_THREADS / 8 * RT_PASS;   // value rows per CTA
 
-template <typename T>
-__global__ void __launch_bounds__(RT_THREADS) k_rec_serial(const __grid_constant__ RecParams p) {
-    __shared__ __align__(16) float ks[RT_TOK][REC_HD], qs[RT_TOK][REC_HD];
-    __shared__ float vs[RT_TOK][RT_ROWS], os[RT_TOK][RT_ROWS], gs[RT_TOK], bs[RT_TOK];
-    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, sub = lane & 7, rq = lane >> 3;
-    const int seq = blockIdx.z, h = blockIdx.y, row0 = blockIdx.x * RT_ROWS;
-    const int32_t beg = p.cu ? p.cu[seq] : seq * p.T, end = p.cu ? p.cu[seq + 1] : beg + p.T;
-    if (beg < 0 || end > p.n_rows || beg > end) {
-        if (tid == 0) atomicOr(p.status, ST_BAD_INDEX);
-        return;
-    }
-    if (beg == end) return;
+template <int T>
+__global__ void __launch_bounds__(RT_THREADS) k_rec_step(const __grid_constant__ RecParams p) {
+    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, sub = lane & 7;
+    const int seq = blockIdx.z, h = blockIdx.y, row0 = blockIdx.x * RT_ROWS + wid * 4 * RT_PASS + (lane >> 3);   // and 4 a rows on
     const int hk = h / (p.n_head / p.n_head_k);
-    const int64_t head_off = ((int64_t)h * REC_HD + row0) * REC_HD;
-    float *S0 = reinterpret_cast<float *>(p.state + (int64_t)p.slot[seq] * p.slot_bytes) + head_off;
-    float S[RT_PASS][16];
+    const int64_t off = ((int64_t)h * REC_HD + row0) * REC_HD + sub * 4, r0 = (int64_t)seq * T;
+    float *S0 = reinterpret_cast<float *>(p.state + (int64_t)p.slot[seq] * p.slot_bytes) + off;
+    float4 S[RT_PASS][4];
 #pragma unroll
-    for (int a = 0; a < RT_PASS; a++) {
-        const int row = (a * 4 + wid) * 4 + rq;
+    for (int a = 0; a < RT_PASS; a++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) S[a][j] = *reinterpret_cast<const float4 *>(S0 + a * 4 * REC_HD + j * 32);
+    const float *k = static_cast<const float *>(p.k) + r0 * p.k_stride + hk * REC_HD + sub * 4;
+    const float *q = static_cast<const float *>(p.q) + r0 * p.q_stride + hk * REC_HD + sub * 4;
+    const float *v = static_cast<const float *>(p.v) + r0 * p.v_stride + h * REC_HD + row0;
+    float4 kf[T][4], qf[T][4];
+    float vf[T][RT_PASS], g[T], b[T];
+#pragma unroll
+    for (int t = 0; t < T; t++) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const float4 u = *reinterpret_cast<const float4 *>(S0 + row * REC_HD + (sub + 8 * j) * 4);
-            S[a][4 * j] = u.x; S[a][4 * j + 1] = u.y; S[a][4 * j + 2] = u.z; S[a][4 * j + 3] = u.w;
+            kf[t][j] = *reinterpret_cast<const float4 *>(k + t * p.k_stride + j * 32);
+            qf[t][j] = *reinterpret_cast<const float4 *>(q + t * p.q_stride + j * 32);
         }
+#pragma unroll
+        for (int a = 0; a < RT_PASS; a++) vf[t][a] = v[t * p.v_stride + a * 4];
+        g[t] = p.g[(r0 + t) * p.n_head + h];
+        b[t] = p.beta ? p.beta[(r0 + t) * p.n_head + h] : 0.0f;
     }
     auto store_state = [&](float *dst) {
 #pragma unroll
+        for (int a = 0; a < RT_PASS; a++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) *reinterpret_cast<float4 *>(dst + a * 4 * REC_HD + j * 32) = S[a][j];
+    };
+    auto back = [&](int s) {   // rollback snapshot s - 1: the state s tokens back
+        return reinterpret_cast<float *>(p.back + ((int64_t)p.slot[seq] * p.n_rollback + s - 1) * p.slot_bytes) + off;
+    };
+    if (T <= p.n_save) store_state(back(T));
+    float *out = static_cast<float *>(p.out) + (r0 * p.n_head + h) * REC_HD + row0;
+#pragma unroll
+    for (int t = 0; t < T; t++) {
+        const float eg = expf(g[t]);
+#pragma unroll
         for (int a = 0; a < RT_PASS; a++) {
-            const int row = (a * 4 + wid) * 4 + rq;
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                *reinterpret_cast<float4 *>(dst + row * REC_HD + (sub + 8 * j) * 4) =
-                    make_float4(S[a][4 * j], S[a][4 * j + 1], S[a][4 * j + 2], S[a][4 * j + 3]);
-        }
-    };
-    auto back_slab = [&](int s) {   // rollback snapshot s - 1: the state s tokens back
-        return reinterpret_cast<float *>(p.back + ((int64_t)p.slot[seq] * p.n_rollback + s - 1) * p.slot_bytes) + head_off;
-    };
-    if (end - beg <= p.n_save) store_state(back_slab(end - beg));
-    const T *q = static_cast<const T *>(p.q) + (int64_t)hk * REC_HD, *k = static_cast<const T *>(p.k) + (int64_t)hk * REC_HD;
-    const T *v = static_cast<const T *>(p.v) + (int64_t)h * REC_HD + row0;
-    constexpr int VEC = RecVec<T>::N;
-    for (int32_t t0 = beg; t0 < end; t0 += RT_TOK) {
-        const int nt = min(RT_TOK, end - t0);
-        __syncthreads();
-        for (int e = tid; e < nt * (REC_HD / VEC); e += RT_THREADS) {
-            const int t = e / (REC_HD / VEC), c = e % (REC_HD / VEC) * VEC;
-            float f[VEC];
-            RecVec<T>::load(k + (int64_t)(t0 + t) * p.k_stride + c, f);
-#pragma unroll
-            for (int i = 0; i < VEC; i++) ks[t][c + i] = f[i];
-            RecVec<T>::load(q + (int64_t)(t0 + t) * p.q_stride + c, f);
-#pragma unroll
-            for (int i = 0; i < VEC; i++) qs[t][c + i] = f[i];
-        }
-        for (int e = tid; e < nt * (RT_ROWS / VEC); e += RT_THREADS) {
-            const int t = e / (RT_ROWS / VEC), c = e % (RT_ROWS / VEC) * VEC;
-            float f[VEC];
-            RecVec<T>::load(v + (int64_t)(t0 + t) * p.v_stride + c, f);
-#pragma unroll
-            for (int i = 0; i < VEC; i++) vs[t][c + i] = f[i];
-        }
-        if (tid < nt) {
-            gs[tid] = expf(p.g[(int64_t)(t0 + tid) * p.n_head + h]);
-            bs[tid] = p.beta ? p.beta[(int64_t)(t0 + tid) * p.n_head + h] : 0.0f;
-        }
-        __syncthreads();
-        for (int t = 0; t < nt; t++) {
-            float kf[16], qf[16];
+            float u = vf[t][a], d = 0.0f, o = 0.0f;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const float4 a = *reinterpret_cast<const float4 *>(&ks[t][(sub + 8 * j) * 4]);
-                const float4 b = *reinterpret_cast<const float4 *>(&qs[t][(sub + 8 * j) * 4]);
-                kf[4 * j] = a.x; kf[4 * j + 1] = a.y; kf[4 * j + 2] = a.z; kf[4 * j + 3] = a.w;
-                qf[4 * j] = b.x; qf[4 * j + 1] = b.y; qf[4 * j + 2] = b.z; qf[4 * j + 3] = b.w;
+                S[a][j].x *= eg;
+                S[a][j].y *= eg;
+                S[a][j].z *= eg;
+                S[a][j].w *= eg;
             }
-            const float eg = gs[t], be = bs[t];
+            if (p.beta) {
 #pragma unroll
-            for (int a = 0; a < RT_PASS; a++) {
-                const int row = (a * 4 + wid) * 4 + rq;
-                float u = vs[t][row];
-#pragma unroll
-                for (int i = 0; i < 16; i++) S[a][i] *= eg;
-                if (p.beta) {
-                    float d = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 16; i++) d = fmaf(S[a][i], kf[i], d);
-#pragma unroll
-                    for (int m = 4; m; m >>= 1) d += __shfl_xor_sync(0xffffffffu, d, m);
-                    u = be * (u - d);
-                }
-                float o = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    S[a][i] = fmaf(u, kf[i], S[a][i]);
-                    o = fmaf(S[a][i], qf[i], o);
+                for (int j = 0; j < 4; j++) {
+                    d = fmaf(S[a][j].x, kf[t][j].x, d);
+                    d = fmaf(S[a][j].y, kf[t][j].y, d);
+                    d = fmaf(S[a][j].z, kf[t][j].z, d);
+                    d = fmaf(S[a][j].w, kf[t][j].w, d);
                 }
 #pragma unroll
-                for (int m = 4; m; m >>= 1) o += __shfl_xor_sync(0xffffffffu, o, m);
-                if (sub == 0) os[t][row] = o * p.scale;
+                for (int m = 4; m; m >>= 1) d += __shfl_xor_sync(0xffffffffu, d, m);
+                u = b[t] * (u - d);
             }
-            const int back = end - (t0 + t) - 1;   // tokens after this one
-            if (back == 0) store_state(S0);
-            else if (back <= p.n_save) store_state(back_slab(back));
-        }
-        __syncthreads();
-        T *out = static_cast<T *>(p.out) + (int64_t)t0 * p.n_head * REC_HD + (int64_t)h * REC_HD + row0;
-        for (int e = tid; e < nt * (RT_ROWS / VEC); e += RT_THREADS) {
-            const int t = e / (RT_ROWS / VEC), c = e % (RT_ROWS / VEC) * VEC;
-            float f[VEC];
 #pragma unroll
-            for (int i = 0; i < VEC; i++) f[i] = os[t][c + i];
-            RecVec<T>::store(out + (int64_t)t * p.n_head * REC_HD + c, f);
+            for (int j = 0; j < 4; j++) {
+                S[a][j].x = fmaf(u, kf[t][j].x, S[a][j].x);
+                S[a][j].y = fmaf(u, kf[t][j].y, S[a][j].y);
+                S[a][j].z = fmaf(u, kf[t][j].z, S[a][j].z);
+                S[a][j].w = fmaf(u, kf[t][j].w, S[a][j].w);
+                o = fmaf(S[a][j].x, qf[t][j].x, o);
+                o = fmaf(S[a][j].y, qf[t][j].y, o);
+                o = fmaf(S[a][j].z, qf[t][j].z, o);
+                o = fmaf(S[a][j].w, qf[t][j].w, o);
+            }
+#pragma unroll
+            for (int m = 4; m; m >>= 1) o += __shfl_xor_sync(0xffffffffu, o, m);
+            if (sub == 0) out[(int64_t)t * p.n_head * REC_HD + a * 4] = o * p.scale;
         }
+        if (t == T - 1) store_state(S0);
+        else if (T - 1 - t <= p.n_save) store_state(back(T - 1 - t));
     }
+}
+
+cudaError_t launch_rec_step(const RecParams &p, cudaStream_t st) {
+    const dim3 grid(REC_HD / RT_ROWS, p.n_head, p.n_seq);
+    switch (p.T) {
+        case 1: k_rec_step<1><<<grid, RT_THREADS, 0, st>>>(p); break;
+        case 2: k_rec_step<2><<<grid, RT_THREADS, 0, st>>>(p); break;
+        case 3: k_rec_step<3><<<grid, RT_THREADS, 0, st>>>(p); break;
+        default: k_rec_step<4><<<grid, RT_THREADS, 0, st>>>(p); break;
+    }
+    count_launches(1);
+    return cudaGetLastError();
 }
 
 // ------------------------------------------------------------------------ chunked linear attention
@@ -423,11 +433,6 @@ __device__ __forceinline__ void row_scales(const float (&x)[N][4], float &s0, fl
     s1 = pow2_scale<12>(quad_max(m1), i1);
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void rk_cp16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -1088,12 +1093,6 @@ __global__ void __launch_bounds__(RK_THREADS, 1) k_rec_chunk(const __grid_consta
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(RK_CHAIN_REGS));
         rk_chain<DELTA>(p, rk_sm, seq, h, row0, beg, end);
     }
-}
-
-cudaError_t launch_rec_step(const RecParams &p, cudaStream_t st) {
-    k_rec_serial<float><<<dim3(REC_HD / RT_ROWS, p.n_head, p.n_seq), RT_THREADS, 0, st>>>(p);
-    count_launches(1);
-    return cudaGetLastError();
 }
 
 cudaError_t launch_rec_chunk(const RecParams &p, cudaStream_t st) {
