@@ -100,38 +100,52 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ void rk_cp16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ float rcp(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
-constexpr int RC_AHEAD = 4;   // rows whose loads are in flight ahead of the ones computed
+constexpr int RC_AHEAD = 8;   // rows in flight ahead of the one computed, in shared memory: they cost no registers
 
 template <typename T>
 __global__ void __launch_bounds__(RC_THREADS, 2) k_rec_conv(const __grid_constant__ RecConvParams p) {
+    __shared__ uint4 ring[RC_AHEAD][RC_THREADS];   // a thread reads what it copied: no barrier
+    __shared__ int32_t cu[MAX_SEQ + 1];
     constexpr int VEC = RecVec<T>::N, LANES = 128 / VEC;
     const int per_row = p.channels / VEC;   // a multiple of LANES
     const int64_t id = (int64_t)blockIdx.x * RC_THREADS + threadIdx.x;
     const int64_t blk = id / per_row;
     const int c0 = (int)(id % per_row) * VEC;
     const int32_t r_lo = (int32_t)min((int64_t)p.n_rows, blk * p.rows_per), r_hi = min(p.n_rows, r_lo + p.rows_per);
-    if (r_lo >= r_hi) return;
     const T *x = static_cast<const T *>(p.x) + c0;
     T *y = static_cast<T *>(p.y) + c0;
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(&ring[0][threadIdx.x]);
+    auto fetch = [&](int32_t r) {   // row r (or nothing) into its slot: one group per row
+        if (r < r_hi) rk_cp16(mine + ((r - r_lo) & (RC_AHEAD - 1)) * (RC_THREADS * 16), x + (int64_t)r * p.x_stride);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int k = 0; k < RC_AHEAD; k++) fetch(r_lo + k);
+    for (int i = threadIdx.x; i <= p.n_seq; i += RC_THREADS) cu[i] = p.cu[i];
     float w[VEC][4];
 #pragma unroll
     for (int e = 0; e < VEC; e++) {
         const float4 u = __ldg(reinterpret_cast<const float4 *>(p.w) + c0 + e);
         w[e][0] = u.x; w[e][1] = u.y; w[e][2] = u.z; w[e][3] = u.w;
     }
+    __syncthreads();
     const bool norm = c0 < p.n_norm;
     const float max_inv = 1.0f / p.eps;
     const unsigned lanes = LANES == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
     for (int32_t r = r_lo; r < r_hi;) {
         int32_t beg, end;   // rows of the sequence
-        const int i = rec_find(p.cu, p.n_seq, p.n_rows, r, beg, end);
+        const int i = rec_find(cu, p.n_seq, p.n_rows, r, beg, end);
         if (i < 0) {        // a row of no sequence (of this launch)
+            fetch(r + RC_AHEAD);
             r++;
             continue;
         }
@@ -171,20 +185,15 @@ __global__ void __launch_bounds__(RC_THREADS, 2) k_rec_conv(const __grid_constan
             }
         }
         const int32_t lim = min(end, r_hi);
-        const T *xr = x + (int64_t)r * p.x_stride;
         T *yr = y + (int64_t)r * p.channels;
-        uint4 next[RC_AHEAD];
+        for (; r < lim; r += 4) {
 #pragma unroll
-        for (int k = 0; k < RC_AHEAD; k++)
-            if (r + k < lim) next[k] = *reinterpret_cast<const uint4 *>(xr + k * p.x_stride);
-        for (; r < lim; r += RC_AHEAD) {
-            xr += RC_AHEAD * p.x_stride;
-#pragma unroll
-            for (int k = 0; k < RC_AHEAD; k++) {
+            for (int k = 0; k < 4; k++) {
                 if (r + k >= lim) break;
                 float (&h0)[VEC] = h[k & 3], (&h1)[VEC] = h[(k + 1) & 3], (&h2)[VEC] = h[(k + 2) & 3], (&v)[VEC] = h[(k + 3) & 3];
-                RecVec<T>::unpack(next[k], v);
-                if (r + RC_AHEAD + k < lim) next[k] = *reinterpret_cast<const uint4 *>(xr + k * p.x_stride);
+                asm volatile("cp.async.wait_group %0;" ::"n"(RC_AHEAD - 1) : "memory");
+                RecVec<T>::unpack(ring[(r + k - r_lo) & (RC_AHEAD - 1)][threadIdx.x], v);
+                fetch(r + k + RC_AHEAD);
                 float o[VEC], ss = 0.0f;
 #pragma unroll
                 for (int e = 0; e < VEC; e++) {
@@ -209,16 +218,25 @@ __global__ void __launch_bounds__(RC_THREADS, 2) k_rec_conv(const __grid_constan
         }
         r = lim;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 cudaError_t launch_rec_conv(RecConvParams &p, bool bf16, int num_sms, cudaStream_t st) {
-    const int per_row = p.channels / (bf16 ? 8 : 4);
-    // rows per thread: as many as leave about 1024 threads per SM, at most 32 (three more rows are
-    // read at the head of each walk)
-    const int64_t want = (int64_t)num_sms * 1024;
-    p.rows_per = (int32_t)std::min<int64_t>(32, std::max<int64_t>(1, (int64_t)p.n_rows * per_row / want));
-    const int64_t threads = (int64_t)((p.n_rows + p.rows_per - 1) / p.rows_per) * per_row;
-    const unsigned grid = (unsigned)((threads + RC_THREADS - 1) / RC_THREADS);
+    const int64_t per_row = p.channels / (bf16 ? 8 : 4), slots = 2 * num_sms;   // CTAs resident at once
+    auto grid_of = [&](int64_t r) { return ((p.n_rows + r - 1) / r * per_row + RC_THREADS - 1) / RC_THREADS; };
+    // Rows per thread: one while a wave of CTAs holds them all, else what makes waves times rows least, with the
+    // start of a walk (its sequence, the three rows before it) counted as eight rows.
+    int64_t best = 1;
+    if (grid_of(1) > slots)
+        for (int64_t r = 4, least = INT64_MAX; r <= 64; r += 4) {
+            const int64_t cost = (grid_of(r) + slots - 1) / slots * (r + 8);
+            if (cost < least) {
+                least = cost;
+                best = r;
+            }
+        }
+    p.rows_per = (int32_t)best;
+    const unsigned grid = (unsigned)grid_of(best);
     if (bf16) k_rec_conv<__nv_bfloat16><<<grid, RC_THREADS, 0, st>>>(p);
     else k_rec_conv<float><<<grid, RC_THREADS, 0, st>>>(p);
     count_launches(1);
@@ -433,9 +451,6 @@ __device__ __forceinline__ void row_scales(const float (&x)[N][4], float &s0, fl
     s1 = pow2_scale<12>(quad_max(m1), i1);
 }
 
-__device__ __forceinline__ void rk_cp16(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 // Sixteen words of bf16 pairs, four lanes holding a row of 128 (lane l its 16-byte chunks l, l + 4, l + 8, l + 12).
 // Bits of the row's largest magnitude (a NaN is above infinity).
 __device__ __forceinline__ uint32_t rk_row_max(const uint4 (&u)[4]) {
