@@ -346,7 +346,7 @@ struct RecParams {
     int32_t slot[MAX_SEQ];
 };
 cudaError_t launch_rec_step(const RecParams &p, cudaStream_t st);    // F32, a few tokens per sequence
-cudaError_t launch_rec_chunk(const RecParams &p, cudaStream_t st);   // bf16, ragged prompts
+cudaError_t launch_rec_chunk(const RecParams &p, cudaStream_t st);   // bf16, ragged prompts (qkv_rec_chunk.cu)
 
 // ---- host side shared by the engine and the saved-sequence store (qkv_store.cpp) ---------------
 // Sets the engine's last error (qkv_last_error) to msg and returns st.

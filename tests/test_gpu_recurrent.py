@@ -158,6 +158,30 @@ def test_chunk(cuda, qkvlib, lengths, H, Hk, delta):
     assert bool((out[rows:] == 7.0).all()) and torch.equal(eng.rec_state(0)[0], S0[0])   # rows and slots of nobody
 
 
+def test_chunk_many_sequences(cuda, qkvlib):
+    """More sequences than a launch takes, more heads and sequences than the GPU holds at once."""
+    lengths = [(37 * i) % 131 for i in range(70)]
+    eng = rec_engine(qkvlib, 4, 1, n_slots=70)
+    S0 = fill(eng, 25)
+    q, k, v, g, beta = inputs(26, sum(lengths), 4, 1, torch.bfloat16, decay=0.05)
+    out = torch.empty(sum(lengths), 4, HD, dtype=torch.bfloat16, device="cuda")
+    slots = [(i * 11) % 70 for i in range(70)]
+    eng.rec_chunk(0, slots, offsets(lengths), q, k, v, g, beta, SCALE, out)
+    check_chunk(eng, S0, slots, lengths, q, k, v, g, beta, out)
+    assert eng.device_status() == 0
+
+
+def test_chunk_growing_state(cuda, qkvlib):
+    """g > 0 in one chunk: a growing state, token by token."""
+    eng = rec_engine(qkvlib, 2, 1, n_slots=1)
+    S0 = fill(eng, 27)
+    q, k, v, g, beta = inputs(28, 300, 2, 1, torch.bfloat16, decay=0.05)
+    g[130:135] = 0.5
+    out = torch.empty(300, 2, HD, dtype=torch.bfloat16, device="cuda")
+    eng.rec_chunk(0, [0], offsets([300]), q, k, v, g, beta, SCALE, out)
+    check_chunk(eng, S0, [0], [300], q, k, v, g, beta, out)
+
+
 @pytest.mark.parametrize("decay", [0.0, 1e-4, 3.0, 60.0])
 def test_chunk_decays(cuda, qkvlib, decay):
     """No decay at all, and decays whose sums over a chunk are far below the smallest exponent."""
