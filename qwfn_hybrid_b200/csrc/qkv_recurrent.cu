@@ -29,9 +29,10 @@ __device__ __forceinline__ int rec_find(const int32_t *__restrict__ cu, int n_se
 // q or k) are then divided by max(|y|_2, eps).  Bound by bytes: each row in and out once.
 // A thread owns VEC channels (16 bytes of a row) and walks R rows with the last three rows in
 // registers; 128 channels are 128 / VEC adjacent lanes, so the norm is a few shuffles.  The thread
-// that meets a sequence's first row has read the history, so it also writes the new one (from the
-// sequence's last three rows) and, for rollbacks, the ones after fewer rows: no second launch and no
-// thread waits for another.
+// that meets a sequence's first row computes its first three rows, however many of them its walk
+// holds, and a walk that starts in the second or third leaves those out: so one thread alone reads a
+// channel's history, and it also writes the new one (from the sequence's last three rows) and, for
+// rollbacks, the ones after fewer rows.  No second launch, and no thread waits for another.
 template <typename T> struct RecVec;
 template <> struct RecVec<float> {
     static constexpr int N = 4;
@@ -108,14 +109,109 @@ __device__ __forceinline__ float rcp(float x) {
     return y;
 }
 
+// The lanes of a warp that hold the thread's head of 128 channels.
+template <typename T>
+__device__ __forceinline__ unsigned rec_head_lanes() { return RecVec<T>::N == 4 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16); }
+// One row of a thread's channels: the three rows before it, the row itself, the taps.
+template <typename T>
+__device__ __forceinline__ void rec_conv_row(const float (&h0)[RecVec<T>::N], const float (&h1)[RecVec<T>::N], const float (&h2)[RecVec<T>::N],
+                                             const float (&v)[RecVec<T>::N], const float (&w)[RecVec<T>::N][4], bool norm, unsigned lanes, float max_inv, T *y) {
+    constexpr int VEC = RecVec<T>::N, LANES = 128 / VEC;
+    float o[VEC], ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < VEC; e++) {
+        float a = v[e] * w[e][3];
+        a = fmaf(h0[e], w[e][0], a);
+        a = fmaf(h1[e], w[e][1], a);
+        a = fmaf(h2[e], w[e][2], a);
+        o[e] = a * rcp(1.0f + ex2(a * -1.4426950408889634f));
+        ss = fmaf(o[e], o[e], ss);
+    }
+    if (norm) {   // the lanes of a head walk the same rows: all of them are here
+#pragma unroll
+        for (int m = LANES / 2; m; m >>= 1) ss += __shfl_xor_sync(lanes, ss, m);
+        float inv = rsqrtf(ss);
+        if (inv > max_inv) inv = max_inv;   // (a NaN stays)
+#pragma unroll
+        for (int e = 0; e < VEC; e++) o[e] *= inv;
+    }
+    RecVec<T>::store(y, o);
+}
+// The rows before row r of the sequence [beg, end) into h: of the sequence itself, or at r = beg the history; then
+// also the history (and, for rollbacks, the ones some rows back) as it will be after the sequence's rows.
+template <typename T>
+__device__ __forceinline__ void rec_conv_enter(const RecConvParams &p, const T *x, int c0, int slot, int32_t r, int32_t beg, int32_t end,
+                                               float (&h)[RC_HIST + 1][RecVec<T>::N]) {
+    constexpr int VEC = RecVec<T>::N;
+    if (r != beg) {
+#pragma unroll
+        for (int j = 0; j < RC_HIST; j++) RecVec<T>::load(x + (int64_t)(r - RC_HIST + j) * p.x_stride, h[j]);
+        return;
+    }
+    float *state = reinterpret_cast<float *>(p.state + (int64_t)slot * p.slot_bytes) + (int64_t)c0 * RC_HIST;
+    float flat[RC_HIST * VEC], old[RC_HIST][VEC];
+#pragma unroll
+    for (int k = 0; k < RC_HIST * VEC / 4; k++) {
+        const float4 u = reinterpret_cast<const float4 *>(state)[k];
+        flat[4 * k] = u.x; flat[4 * k + 1] = u.y; flat[4 * k + 2] = u.z; flat[4 * k + 3] = u.w;
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; e++)
+#pragma unroll
+        for (int j = 0; j < RC_HIST; j++) h[j][e] = old[j][e] = flat[e * RC_HIST + j];
+    for (int s = 1; s <= min(p.n_save, end - beg); s++)
+        rec_conv_hist<T, VEC>(p, x, beg, end - s, old,
+                              reinterpret_cast<float *>(p.back + ((int64_t)slot * p.n_rollback + s - 1) * p.slot_bytes) + (int64_t)c0 * RC_HIST);
+    rec_conv_hist<T, VEC>(p, x, beg, end, old, state);
+}
+
+// The few rows of decode steps: a thread per 16 bytes of a row.
+template <typename T>
+constexpr int RC_STEP_CTAS = sizeof(T) == 4 ? 4 : 2;   // resident per SM
+template <typename T>
+__global__ void __launch_bounds__(RC_THREADS, RC_STEP_CTAS<T>) k_rec_conv_rows(const __grid_constant__ RecConvParams p) {
+    __shared__ int32_t cu[MAX_SEQ + 1];
+    constexpr int VEC = RecVec<T>::N;
+    const int per_row = p.channels / VEC;
+    const int64_t id = (int64_t)blockIdx.x * RC_THREADS + threadIdx.x;
+    const int32_t r = (int32_t)min((int64_t)p.n_rows, id / per_row);
+    const int c0 = (int)(id % per_row) * VEC;
+    const T *x = static_cast<const T *>(p.x) + c0;
+    const bool in = r < p.n_rows;
+    float w[VEC][4], h[RC_HIST + 1][VEC];   // rows r - 3 .. r
+    if (in) RecVec<T>::load(x + (int64_t)r * p.x_stride, h[3]);
+#pragma unroll
+    for (int e = 0; e < VEC; e++) {
+        const float4 u = __ldg(reinterpret_cast<const float4 *>(p.w) + c0 + e);
+        w[e][0] = u.x; w[e][1] = u.y; w[e][2] = u.z; w[e][3] = u.w;
+    }
+    for (int i = threadIdx.x; i <= p.n_seq; i += RC_THREADS) cu[i] = p.cu[i];
+    __syncthreads();
+    if (!in) return;
+    int32_t beg, end;
+    const int i = rec_find(cu, p.n_seq, p.n_rows, r, beg, end);
+    // A row of no sequence (of this launch), or the second or third of one: all lanes of the head leave.
+    if (i < 0 || (r > beg && r < beg + RC_HIST)) return;
+    rec_conv_enter<T>(p, x, c0, p.slot[i], r, beg, end, h);
+    T *y = static_cast<T *>(p.y) + (int64_t)r * p.channels + c0;
+    const int n = r == beg ? min(RC_HIST, end - beg) : 1;
+#pragma unroll
+    for (int k = 0; k < RC_HIST; k++) {
+        if (k >= n) break;
+        if (k) RecVec<T>::load(x + (int64_t)(r + k) * p.x_stride, h[(k + 3) & 3]);
+        rec_conv_row<T>(h[k & 3], h[(k + 1) & 3], h[(k + 2) & 3], h[(k + 3) & 3], w, c0 < p.n_norm, rec_head_lanes<T>(), 1.0f / p.eps,
+                        y + (int64_t)k * p.channels);
+    }
+}
+
 constexpr int RC_AHEAD = 8;   // rows in flight ahead of the one computed, in shared memory: they cost no registers
 
 template <typename T>
 __global__ void __launch_bounds__(RC_THREADS, 2) k_rec_conv(const __grid_constant__ RecConvParams p) {
     __shared__ uint4 ring[RC_AHEAD][RC_THREADS];   // a thread reads what it copied: no barrier
     __shared__ int32_t cu[MAX_SEQ + 1];
-    constexpr int VEC = RecVec<T>::N, LANES = 128 / VEC;
-    const int per_row = p.channels / VEC;   // a multiple of LANES
+    constexpr int VEC = RecVec<T>::N;
+    const int per_row = p.channels / VEC;   // a multiple of the 128 / VEC lanes of a head
     const int64_t id = (int64_t)blockIdx.x * RC_THREADS + threadIdx.x;
     const int64_t blk = id / per_row;
     const int c0 = (int)(id % per_row) * VEC;
@@ -139,51 +235,18 @@ __global__ void __launch_bounds__(RC_THREADS, 2) k_rec_conv(const __grid_constan
     __syncthreads();
     const bool norm = c0 < p.n_norm;
     const float max_inv = 1.0f / p.eps;
-    const unsigned lanes = LANES == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
+    const unsigned lanes = rec_head_lanes<T>();
     for (int32_t r = r_lo; r < r_hi;) {
         int32_t beg, end;   // rows of the sequence
         const int i = rec_find(cu, p.n_seq, p.n_rows, r, beg, end);
-        if (i < 0) {        // a row of no sequence (of this launch)
+        if (i < 0 || (r > beg && r < beg + RC_HIST)) {   // of no sequence (of this launch), or of the walk that holds its first row
             fetch(r + RC_AHEAD);
             r++;
             continue;
         }
         float h[RC_HIST + 1][VEC];   // rows r - 3 .. r
-        {
-            float *state = reinterpret_cast<float *>(p.state + (int64_t)p.slot[i] * p.slot_bytes) + (int64_t)c0 * RC_HIST;
-            float old[RC_HIST][VEC];
-            if (r - beg < RC_HIST) {
-                float flat[RC_HIST * VEC];
-#pragma unroll
-                for (int k = 0; k < RC_HIST * VEC / 4; k++) {
-                    const float4 u = reinterpret_cast<const float4 *>(state)[k];
-                    flat[4 * k] = u.x; flat[4 * k + 1] = u.y; flat[4 * k + 2] = u.z; flat[4 * k + 3] = u.w;
-                }
-#pragma unroll
-                for (int e = 0; e < VEC; e++)
-#pragma unroll
-                    for (int j = 0; j < RC_HIST; j++) old[j][e] = flat[e * RC_HIST + j];
-            }
-#pragma unroll
-            for (int j = 0; j < RC_HIST; j++) {
-                const int32_t q = r - RC_HIST + j;
-                if (q >= beg) {
-                    RecVec<T>::load(x + (int64_t)q * p.x_stride, h[j]);
-                } else {
-                    const int32_t k = q - beg + RC_HIST;
-#pragma unroll
-                    for (int e = 0; e < VEC; e++) h[j][e] = k == 0 ? old[0][e] : k == 1 ? old[1][e] : old[2][e];
-                }
-            }
-            if (r == beg) {
-                for (int s = 1; s <= min(p.n_save, end - beg); s++)
-                    rec_conv_hist<T, VEC>(p, x, beg, end - s, old,
-                                          reinterpret_cast<float *>(p.back + ((int64_t)p.slot[i] * p.n_rollback + s - 1) * p.slot_bytes) +
-                                              (int64_t)c0 * RC_HIST);
-                rec_conv_hist<T, VEC>(p, x, beg, end, old, state);
-            }
-        }
-        const int32_t lim = min(end, r_hi);
+        rec_conv_enter<T>(p, x, c0, p.slot[i], r, beg, end, h);
+        const int32_t lim = min(end, r == beg ? max(r_hi, beg + RC_HIST) : r_hi);
         T *yr = y + (int64_t)r * p.channels;
         for (; r < lim; r += 4) {
 #pragma unroll
@@ -191,27 +254,10 @@ __global__ void __launch_bounds__(RC_THREADS, 2) k_rec_conv(const __grid_constan
                 if (r + k >= lim) break;
                 float (&h0)[VEC] = h[k & 3], (&h1)[VEC] = h[(k + 1) & 3], (&h2)[VEC] = h[(k + 2) & 3], (&v)[VEC] = h[(k + 3) & 3];
                 asm volatile("cp.async.wait_group %0;" ::"n"(RC_AHEAD - 1) : "memory");
-                RecVec<T>::unpack(ring[(r + k - r_lo) & (RC_AHEAD - 1)][threadIdx.x], v);
+                if (r + k < r_hi) RecVec<T>::unpack(ring[(r + k - r_lo) & (RC_AHEAD - 1)][threadIdx.x], v);
+                else RecVec<T>::load(x + (int64_t)(r + k) * p.x_stride, v);   // past the walk: a sequence's second or third row
                 fetch(r + k + RC_AHEAD);
-                float o[VEC], ss = 0.0f;
-#pragma unroll
-                for (int e = 0; e < VEC; e++) {
-                    float a = v[e] * w[e][3];
-                    a = fmaf(h0[e], w[e][0], a);
-                    a = fmaf(h1[e], w[e][1], a);
-                    a = fmaf(h2[e], w[e][2], a);
-                    o[e] = a * rcp(1.0f + ex2(a * -1.4426950408889634f));
-                    ss = fmaf(o[e], o[e], ss);
-                }
-                if (norm) {   // the lanes of a head walk the same rows: all of them are here
-#pragma unroll
-                    for (int m = LANES / 2; m; m >>= 1) ss += __shfl_xor_sync(lanes, ss, m);
-                    float inv = rsqrtf(ss);
-                    if (inv > max_inv) inv = max_inv;   // (a NaN stays)
-#pragma unroll
-                    for (int e = 0; e < VEC; e++) o[e] *= inv;
-                }
-                RecVec<T>::store(yr, o);
+                rec_conv_row<T>(h0, h1, h2, v, w, norm, lanes, max_inv, yr);
                 yr += p.channels;
             }
         }
@@ -221,12 +267,19 @@ __global__ void __launch_bounds__(RC_THREADS, 2) k_rec_conv(const __grid_constan
 }
 
 cudaError_t launch_rec_conv(RecConvParams &p, bool bf16, int num_sms, cudaStream_t st) {
-    const int64_t per_row = p.channels / (bf16 ? 8 : 4), slots = 2 * num_sms;   // CTAs resident at once
+    const int64_t per_row = p.channels / (bf16 ? 8 : 4);
     auto grid_of = [&](int64_t r) { return ((p.n_rows + r - 1) / r * per_row + RC_THREADS - 1) / RC_THREADS; };
-    // Rows per thread: one while a wave of CTAs holds them all, else what makes waves times rows least, with the
-    // start of a walk (its sequence, the three rows before it) counted as eight rows.
-    int64_t best = 1;
-    if (grid_of(1) > slots)
+    if (grid_of(1) <= (int64_t)num_sms * (bf16 ? RC_STEP_CTAS<__nv_bfloat16> : RC_STEP_CTAS<float>)) {
+        // One wave of CTAs holds a thread per 16 bytes: the kernel without the ring of copies, which needs fewer
+        // registers and no start of a walk (64 rows of 8192 F32 channels: 6.1 us against 9.9 for walks of four).
+        p.rows_per = 1;
+        if (bf16) k_rec_conv_rows<__nv_bfloat16><<<(unsigned)grid_of(1), RC_THREADS, 0, st>>>(p);
+        else k_rec_conv_rows<float><<<(unsigned)grid_of(1), RC_THREADS, 0, st>>>(p);
+    } else {
+        // Rows per thread: what makes waves times rows least, with the start of a walk (its sequence, the three
+        // rows before it) counted as eight rows.
+        int64_t best = 4;
+        const int64_t slots = 2 * num_sms;   // CTAs resident at once
         for (int64_t r = 4, least = INT64_MAX; r <= 64; r += 4) {
             const int64_t cost = (grid_of(r) + slots - 1) / slots * (r + 8);
             if (cost < least) {
@@ -234,10 +287,10 @@ cudaError_t launch_rec_conv(RecConvParams &p, bool bf16, int num_sms, cudaStream
                 best = r;
             }
         }
-    p.rows_per = (int32_t)best;
-    const unsigned grid = (unsigned)grid_of(best);
-    if (bf16) k_rec_conv<__nv_bfloat16><<<grid, RC_THREADS, 0, st>>>(p);
-    else k_rec_conv<float><<<grid, RC_THREADS, 0, st>>>(p);
+        p.rows_per = (int32_t)best;
+        if (bf16) k_rec_conv<__nv_bfloat16><<<(unsigned)grid_of(best), RC_THREADS, 0, st>>>(p);
+        else k_rec_conv<float><<<(unsigned)grid_of(best), RC_THREADS, 0, st>>>(p);
+    }
     count_launches(1);
     return cudaGetLastError();
 }

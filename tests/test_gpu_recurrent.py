@@ -298,6 +298,28 @@ def test_conv(cuda, qkvlib, lengths, channels, n_norm, dtype):
     assert bool((y[rows:] == 7.0).all()) and torch.equal(h1[0], h0[0])
 
 
+@pytest.mark.parametrize("ahead,dtype", [(1, torch.bfloat16), (2, torch.bfloat16), (2, torch.float32)])
+def test_conv_history_is_read_before_it_is_replaced(cuda, qkvlib, ahead, dtype):
+    """Sequences that start one or two rows before a multiple of four, those among them where a wave of thread blocks
+    ends: a thread whose rows begin just behind a sequence's start needs what the start replaces."""
+    channels, n = 8192, 24
+    step = 4 * (2 * torch.cuda.get_device_properties(0).multi_processor_count * 256 * 8 // channels)
+    lengths = [step - ahead] + [step] * (n - 1)
+    rows, gen = sum(lengths), torch.Generator().manual_seed(35)
+    engs = [rec_engine(qkvlib, 2, 1, n_slots=n, channels=channels, layers=1) for _ in range(2)]
+    for e in engs:
+        fill(e, 36, kind=1, scale=1.0)
+    x = torch.randn(rows, channels, generator=gen).to(dtype).cuda()
+    w = torch.randn(channels, 4, generator=gen).cuda()
+    y, alone = torch.empty_like(x), torch.empty_like(x)
+    engs[0].rec_conv(0, list(range(n)), offsets(lengths), x, w, y, n_norm=4096)
+    at = 0
+    for i, m in enumerate(lengths):   # a sequence's first three rows as a call of their own
+        engs[1].rec_conv(0, [i], offsets([3]), x[at:at + 3], w, alone[at:at + 3], n_norm=4096)
+        assert torch.equal(y[at:at + 3], alone[at:at + 3]), f"sequence {i}"
+        at += m
+
+
 def test_conv_zero_head(cuda, qkvlib):
     eng = rec_engine(qkvlib, 2, 1, n_slots=1, channels=256)
     eng.reset(0)
