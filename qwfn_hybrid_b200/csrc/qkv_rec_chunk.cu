@@ -214,6 +214,7 @@ __device__ __forceinline__ void rk_wait(uint64_t *bar, uint32_t parity, RkCtl *c
 }
 
 // ---- producers
+__device__ __forceinline__ void rk_prefetch(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ void rk_cp16_zero(uint32_t dst, const void *src, bool ok) {   // zeros unless ok (src is not read then)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16u : 0u) : "memory");
 }
@@ -342,6 +343,15 @@ __device__ __forceinline__ void rk_produce(const RecParams &p, uint8_t *sm, RkCt
                 const uint32_t off = su + (ch >> 3) * RK_KSUB + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
                 rk_cp16_zero(off + RK_KQ, kp + at * p.k_stride, ok);
                 rk_cp16_zero(off + RK_KQ + 8192, qp + at * p.q_stride, ok);
+            }
+        }
+        {   // the group's next chunk on its way into L2
+            const int32_t r = t0 + RK_GROUPS * RK_C + (tid >> 1);
+            if (r < end) {
+                const int o = (tid & 1) * 64;
+                rk_prefetch(static_cast<const __nv_bfloat16 *>(p.k) + (int64_t)r * p.k_stride + (int64_t)hk * REC_HD + o);
+                rk_prefetch(static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)r * p.q_stride + (int64_t)hk * REC_HD + o);
+                rk_prefetch(static_cast<const __nv_bfloat16 *>(p.v) + (int64_t)r * p.v_stride + (int64_t)h * REC_HD + o);
             }
         }
         if (tid == 0) cf[CF_N * RK_C + 1] = 0.0f;
