@@ -12,15 +12,19 @@
 // registers, thread (row, half) holding 64 keys of a value row, and every product has the value rows as its
 // M = 128, so that its A operand is written to tensor memory by the thread that has just read the last product from
 // there (lane = value row: no shuffles, no shared memory); B is k, q, T and P in shared memory as they are.  Per
-// chunk: [X | O] = S [k; q]^T, U = R T^T, S += (w U) k (k as an MN-major operand, the same bytes), O += U P^T.  A warp of
-// its own issues the products, so that no other waits for the tensor cores to take one.
+// chunk: X = S k^T, U = R T^T, O = S q^T, S += (w U) k (k as an MN-major operand, the same bytes), O += U P^T.  A warp of
+// its own issues the products, so that no other waits for the tensor cores to take one; S q^T goes behind what the
+// chain waits for (beside X, as one product of 128 columns, a 16K prompt takes 4% longer).  The chain reads a chunk's O while
+// the next chunk's X is made, and stores it while that chunk's part of S is made.
+//
+// Where the sequences are more than two, the CTAs take the longest first (24 prompts of 24001 rows: 656 against 690 us).
 //
 // Precision.  k and q are exact in bf16, so S, w U and U enter as sums of bf16 terms (three: 24 bits; two for what
-// only the rounded output sees, as P), and T and R, which meet each other, as two f16 terms of rows scaled to
-// [2^12, 2^13) (22 bits), three products: state and U keep 32-bit accuracy (2 to 5e-7 of the state's norm against
-// 64 bits).  Sums are F32; the state is scaled and added outside the tensor cores (their sums are truncated).  G is
-// summed as pairs of floats: e^(G_i - G_j) needs the difference, not the rounded sums.  The output is
-// rounded to bf16 once.
+// only the rounded output sees, as P; truncated terms, which need no conversion: three of them are the value), and T
+// and R, which meet each other, as two f16 terms of rows scaled to [2^12, 2^13) (22 bits), three products: state and U
+// keep 32-bit accuracy (2 to 5e-7 of the state's norm against 64 bits).  Sums are F32; the state is scaled and added
+// outside the tensor cores (their sums are truncated).  G is summed as pairs of floats: e^(G_i - G_j) needs the
+// difference, not the rounded sums.  The output is rounded to bf16 once.
 //
 // A zero of T or P times a NaN is a NaN, so a chunk with a non-finite input would spread it to earlier
 // tokens; such chunks (and those with g > 0, a growing state, which could leave the range of what is scaled) are
@@ -28,11 +32,11 @@
 //
 // What bounds it: neither bytes nor the tensor cores (60 products of 64 cycles a chunk) but the chain's latency -- four
 // round trips from registers through tensor memory and a product a chunk -- and, beside it on the same
-// schedulers, the producers'.  A chunk takes 6.2 us (delta rule) or 3.7 us; alone the chain takes 4.6 and the
-// producers 4.1 us (delta rule).  A kernel of the same split on mma.sync, 64 value rows per CTA with S as the accumulator
-// that is the next product's A operand, took 5.9 us per chunk and half a head: 5% less where 64 heads or fewer
-// run at once (37 heads x 2 sequences x 1024 tokens: 118 against 114 us), 1.6 to 1.75 times as long where they fill the
-// GPU (768: 1097 against 704 us).
+// schedulers, the producers'.  A chunk takes 5.25 us (delta rule, 16384 tokens: 1345 us) or 3.7 us; alone the
+// producers take 4.1 us (delta rule), and a shorter way to T (blocks of 8, fewer barriers, shorter chains of products)
+// changed nothing.  A kernel of the same split on mma.sync, 64 value rows per CTA with S as the accumulator that is the
+// next product's A operand, took 5.9 us per chunk and half a head, 1.6 to 1.75 times as long where the heads fill the
+// GPU (24 prompts of 24001 rows: 1097 against 656 us).
 #include "qkv_internal.h"
 
 #include <cuda_bf16.h>
@@ -59,11 +63,13 @@ static_assert(RK_COEF + CF_N * RK_C * 4 + 8 <= RK_STAGE, "stage");
 constexpr int RK_PITCH = 20, RK_TILE = 16 * RK_PITCH;
 static_assert(10 * RK_TILE * 4 <= 2 * 8192, "tiles of A in the place of T");
 constexpr int RK_VS = RK_STAGES * RK_STAGE;   // v of one chunk as it is, then the control block
+constexpr int RK_BARS = 5;
 struct RkCtl {
-    uint64_t bar[4];          // products done: X, U, S, O
+    uint64_t bar[RK_BARS];    // products done: X, U, S, O's second part; O's first
     uint64_t scored[RK_GROUPS], read;   // a group's scores are there; their columns have been read
     uint32_t tmem;
     int32_t  abort;
+    int32_t  seq;
     float    scale[128];      // inverse scale of R's first 32 tokens, per value row
 };
 constexpr int RK_CTL = RK_VS + RK_C * REC_HD * 2;
@@ -98,18 +104,20 @@ __device__ __forceinline__ float pow2_scale(float m, float &inv) {
     return __int_as_float(f << 23);
 }
 __device__ __forceinline__ void split_f16(float a, float b, float s, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __floats2half2_rn(a * s, b * s);
-    const float2 f = __half22float2(h);
+    a *= s;
+    b *= s;
+    const __half2 h = __floats2half2_rn(a, b);
     hi = *reinterpret_cast<const uint32_t *>(&h);
-    const __half2 l = __floats2half2_rn(fmaf(a, s, -f.x), fmaf(b, s, -f.y));
+    asm("{\n\t.reg .b16 l, h, m;\n\tmov.b32 {l, h}, %2;\n\tmov.b16 m, 0xBC00;\n\tfma.rn.f32.f16 %0, l, m, %0;\n\tfma.rn.f32.f16 %1, h, m, %1;\n\t}"
+        : "+f"(a), "+f"(b) : "r"(hi));
+    const __half2 l = __floats2half2_rn(a, b);
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
-// The leading bf16 term of two values; they become what is left of them (exactly; both in one instruction).
+// The leading bf16 term (truncated) of two values; they become what is left of them, exactly.
 __device__ __forceinline__ uint32_t take_bf16(float &a, float &b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    const uint32_t w = *reinterpret_cast<const uint32_t *>(&h);
-    asm("{\n\t.reg .b64 x, y, m;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tmov.b64 m, {%4, %4};\n\tfma.rn.f32x2 x, y, m, x;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "+f"(a), "+f"(b) : "f"(__uint_as_float(w << 16)), "f"(__uint_as_float(w & 0xffff0000u)), "f"(-1.0f));
+    const uint32_t w = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+    asm("{\n\t.reg .b16 l, h, m;\n\tmov.b32 {l, h}, %2;\n\tmov.b16 m, 0xBF80;\n\tfma.rn.f32.bf16 %0, l, m, %0;\n\tfma.rn.f32.bf16 %1, h, m, %1;\n\t}"
+        : "+f"(a), "+f"(b) : "r"(w));   // less the term, by a factor of -1
     return w;
 }
 
@@ -583,27 +591,35 @@ __device__ __noinline__ void rk_serial(const RecParams &p, float *S, int h, int 
 
 // The warp that issues the products: of a chunk in the order in which the chain hands their operands over.
 template <bool DELTA>
-__device__ __forceinline__ void rk_issue(uint8_t *sm, RkCtl *ctl, int32_t beg, int32_t end) {
+__device__ __forceinline__ void rk_issue(uint8_t *sm, RkCtl *ctl, int32_t beg, int32_t end, int32_t *status) {
     const uint32_t smu = (uint32_t)__cvta_generic_to_shared(sm), tm = ctl->tmem;
     const bool one = (threadIdx.x & 31) == 0;
     const int n_chunks = (end - beg + RK_C - 1) / RK_C;
+    uint32_t parity = 0;
     for (int c = 0, st = 0; c < n_chunks; c++, st = st == RK_STAGES - 1 ? 0 : st + 1) {
         const uint32_t su = smu + st * RK_STAGE;
         bar_sync(BAR_FULL + st, RK_FULL_N);
         if (reinterpret_cast<const float *>(sm + st * RK_STAGE + RK_COEF)[CF_N * RK_C + 1] != 0.0f) continue;
-        const uint64_t kq = rk_desc(su + RK_KQ + (DELTA ? 0 : 8192), 16), kt = rk_desc(su + RK_KQ, RK_KSUB);
+        const uint64_t kq = rk_desc(su + RK_KQ, 16), kt = rk_desc(su + RK_KQ, RK_KSUB);
         const uint64_t th = rk_desc(su + RK_TH, 16), tl = rk_desc(su + RK_TL, 16), ph = rk_desc(su + RK_PH, 16), pm = rk_desc(su + RK_PM, 16);
         bar_sync(BAR_HAND, RK_HAND_N);
         tc_fence_after();
-        if (one) {   // [X | O] = S [k; q]^T, or O = S q^T
+        auto times_s = [&](uint32_t d, uint64_t b, int terms) {   // S times 64 rows of k or q
 #pragma unroll
-            for (int term = 0; term < (DELTA ? 3 : 2); term++)
+            for (int term = 0; term < terms; term++)
 #pragma unroll
                 for (int kk = 0; kk < 8; kk++)
-                    rk_mma(tm + (DELTA ? TM_X : TM_O1),
-                           tm + (term < 2 ? TM_S + 64 * (kk >> 2) + 32 * term : TM_S2 + 32 * (kk >> 2)) + 8 * (kk & 3),
-                           kq + (((kk >> 2) * RK_KSUB + (kk & 3) * 32) >> 4), rk_idesc(DELTA ? 128 : 64, true, false), term + kk > 0);
-            rk_commit(&ctl->bar[0]);
+                    rk_mma(tm + d, tm + (term < 2 ? TM_S + 64 * (kk >> 2) + 32 * term : TM_S2 + 32 * (kk >> 2)) + 8 * (kk & 3),
+                           b + (((kk >> 2) * RK_KSUB + (kk & 3) * 32) >> 4), rk_idesc(64, true, false), term + kk > 0);
+        };
+        if (one) {
+            if (DELTA) {
+                times_s(TM_X, kq, 3);
+                rk_commit(&ctl->bar[0]);
+            } else {
+                times_s(TM_O1, kq + (8192 >> 4), 2);
+                rk_commit(&ctl->bar[4]);
+            }
         }
         __syncwarp();
         if (DELTA) {
@@ -620,11 +636,15 @@ __device__ __forceinline__ void rk_issue(uint8_t *sm, RkCtl *ctl, int32_t beg, i
                                    (term == 2 ? tl : th) + (((part ? 32 * 128 + 64 : 0) + 32 * ks) >> 4),
                                    rk_idesc(part ? 32 : 64, false, false), term + ks > 0);
                 rk_commit(&ctl->bar[1]);
+                // (not before: the last chunk's output has been read by those who handed R over)
+                times_s(TM_O1, kq + (8192 >> 4), 2);
+                rk_commit(&ctl->bar[4]);
             }
             __syncwarp();
         }
         bar_sync(BAR_HAND, RK_HAND_N);
         tc_fence_after();
+        rk_wait(&ctl->bar[4], parity, ctl, status);   // the last reader of S's terms, which the new part replaces
         if (one) {   // the new part of S
 #pragma unroll
             for (int term = 0; term < 3; term++)
@@ -645,6 +665,7 @@ __device__ __forceinline__ void rk_issue(uint8_t *sm, RkCtl *ctl, int32_t beg, i
             rk_commit(&ctl->bar[3]);
         }
         __syncwarp();
+        parity ^= 1;
     }
 }
 
@@ -687,8 +708,37 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
     uint32_t ow[16];         // the last chunk's output of tokens 32 half .., pairs of tokens, on its way to memory
     int32_t out_t0 = -1;     // that chunk's first token (-1: nothing pending)
     uint32_t ph = 0;         // parity of the products' barriers
+    auto release = [&](int c) {   // chunk c's stage
+        const int next = c + RK_STAGES;
+        if (next < n_chunks) bar_arrive(BAR_EMPTY + next % RK_STAGES * RK_GROUPS + next % RK_GROUPS, RK_EMPTY_N);
+    };
+    auto read_out = [&](int c, uint32_t parity) {   // O of chunk c: scale (e^G S q + P U)
+        const float *cf = reinterpret_cast<const float *>(sm + c % RK_STAGES * RK_STAGE + RK_COEF);
+        rk_wait(&ctl->bar[3], parity, ctl, p.status);
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            float u[16], o[16];
+            tm_ld16(tl + TM_O1 + 32 * half + 16 * b, u);
+            tm_ld16(tl + TM_U + 32 * half + 16 * b, o);
+            tm_wait16(u);
+            tm_wait16(o);
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const float4 cq = *reinterpret_cast<const float4 *>(cf + CF_Q * RK_C + 32 * half + 16 * b + i);
+                const __nv_bfloat162 v0 = __floats2bfloat162_rn(fmaf(cq.x, u[i], p.scale * o[i]), fmaf(cq.y, u[i + 1], p.scale * o[i + 1]));
+                const __nv_bfloat162 v1 = __floats2bfloat162_rn(fmaf(cq.z, u[i + 2], p.scale * o[i + 2]), fmaf(cq.w, u[i + 3], p.scale * o[i + 3]));
+                ow[8 * b + i / 2] = *reinterpret_cast<const uint32_t *>(&v0);
+                ow[8 * b + i / 2 + 1] = *reinterpret_cast<const uint32_t *>(&v1);
+            }
+        }
+        release(c);
+    };
     const int64_t out_row = (int64_t)p.n_head * REC_HD;
+    auto read_last = [&]() {   // with the delta rule a chunk's O is read while the next chunk's X is made
+        if (DELTA && out_t0 >= 0) read_out((out_t0 - beg) / RK_C, ph ^ 1);
+    };
     auto finish_out = [&]() {
+        if (out_t0 < 0) return;
         __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out) + (int64_t)(out_t0 + 32 * half) * out_row + (int64_t)h * REC_HD + row;
         const int n = end - out_t0 - 32 * half;
 #pragma unroll
@@ -702,18 +752,18 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
     for (int c = 0, st = 0; c < n_chunks; c++, st = st == RK_STAGES - 1 ? 0 : st + 1) {
         const int32_t t0 = beg + c * RK_C;
         const float *cf = reinterpret_cast<const float *>(sm + st * RK_STAGE + RK_COEF);
-        asm volatile("cp.async.wait_all;" ::: "memory");   // (this thread's part of v: all see it once X is done)
+        asm volatile("cp.async.wait_all;" ::: "memory");   // (this thread's part of v: all see it behind the barrier)
         bar_sync(BAR_FULL + st, RK_FULL_N);
         if (cf[CF_N * RK_C + 1] != 0.0f) {
-            if (out_t0 >= 0) finish_out();
+            read_last();
+            finish_out();
             store_state();
             bar_sync(BAR_CHAIN, RK_CHAIN);
             load_v(t0 + RK_C);
             if (half == 0) rk_serial<DELTA>(p, S0, h, row, t0, min(end, t0 + RK_C));
             bar_sync(BAR_CHAIN, RK_CHAIN);
             load_state();
-            const int next = c + RK_STAGES;
-            if (next < n_chunks) bar_arrive(BAR_EMPTY + next % RK_STAGES * RK_GROUPS + next % RK_GROUPS, RK_EMPTY_N);
+            release(c);
             continue;
         }
         // S as bf16 terms
@@ -732,12 +782,13 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
             if (DELTA) tm_st8(tl + TM_S2 + 32 * half + 8 * b, w2);
         }
         hand_over(BAR_HAND);
-        if (out_t0 >= 0) finish_out();
+        if (DELTA) read_last();
+        else finish_out();
         // R = beta (v - e^G X), or u = v: tokens 32 half ..
         float X[32];
         const uint16_t *vs = reinterpret_cast<const uint16_t *>(sm + RK_VS) + 32 * half * 128 + row;
-        rk_wait(&ctl->bar[0], ph, ctl, p.status);
         if (DELTA) {
+            rk_wait(&ctl->bar[0], ph, ctl, p.status);
             float mx = 0.0f, inv;
             tm_ld32(tl + TM_X + 32 * half, X);
             tm_wait_ld(X);
@@ -825,6 +876,7 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
             tm_st8(tl + TM_UM + 16 * half + 8 * b, w1);
         }
         hand_over(BAR_HAND_U);
+        if (DELTA) finish_out();
         const float eg = cf[CF_N * RK_C];
         rk_wait(&ctl->bar[2], ph, ctl, p.status);
         if (!DELTA) load_v(t0 + RK_C);   // (every thread has read its part)
@@ -835,31 +887,12 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
 #pragma unroll
             for (int i = 0; i < 32; i++) S[32 * b + i] = fmaf(eg, S[32 * b + i], X[i]);
         }
-        rk_wait(&ctl->bar[3], ph, ctl, p.status);
-#pragma unroll
-        for (int b = 0; b < 2; b++) {   // O: scale (e^G S q + P U)
-            float u[16], o[16];
-            tm_ld16(tl + TM_O1 + 32 * half + 16 * b, u);
-            tm_ld16(tl + TM_U + 32 * half + 16 * b, o);
-            tm_wait16(u);
-            tm_wait16(o);
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const float4 cq = *reinterpret_cast<const float4 *>(cf + CF_Q * RK_C + 32 * half + 16 * b + i);
-                const __nv_bfloat162 v0 = __floats2bfloat162_rn(fmaf(cq.x, u[i], p.scale * o[i]), fmaf(cq.y, u[i + 1], p.scale * o[i + 1]));
-                const __nv_bfloat162 v1 = __floats2bfloat162_rn(fmaf(cq.z, u[i + 2], p.scale * o[i + 2]), fmaf(cq.w, u[i + 3], p.scale * o[i + 3]));
-                ow[8 * b + i / 2] = *reinterpret_cast<const uint32_t *>(&v0);
-                ow[8 * b + i / 2 + 1] = *reinterpret_cast<const uint32_t *>(&v1);
-            }
-        }
-        {
-            const int next = c + RK_STAGES;
-            if (next < n_chunks) bar_arrive(BAR_EMPTY + next % RK_STAGES * RK_GROUPS + next % RK_GROUPS, RK_EMPTY_N);
-        }
+        if (!DELTA) read_out(c, ph);
         out_t0 = t0;
         ph ^= 1;
     }
-    if (out_t0 >= 0) finish_out();
+    read_last();
+    finish_out();
     asm volatile("cp.async.wait_all;" ::: "memory");
     store_state();
 }
@@ -869,7 +902,30 @@ __global__ void __launch_bounds__(RK_THREADS, 1) k_rec_chunk(const __grid_consta
     extern __shared__ uint8_t rk_raw[];
     uint8_t *sm = rk_raw + ((1024 - ((uint32_t)__cvta_generic_to_shared(rk_raw) & 1023)) & 1023);   // swizzled tiles: 1024-byte atoms
     RkCtl *ctl = reinterpret_cast<RkCtl *>(sm + RK_CTL);
-    const int seq = blockIdx.y, h = blockIdx.x;
+    const int h = blockIdx.x;
+    int seq = blockIdx.y;
+    if (gridDim.y > 2) {   // the longest sequences first: the blockIdx.y-th by length
+        if (threadIdx.x < 32) {
+            const int lane = threadIdx.x, n = gridDim.y;
+            auto length = [&](int i) {   // + 1; 0 behind the last sequence (whatever cu holds, each sequence gets one place)
+                if (i >= n) return 0u;
+                const int32_t a = p.cu[i], b = p.cu[i + 1];
+                return b > a ? min((uint32_t)b - (uint32_t)a, 0x7fffffffu) + 1 : 1u;
+            };
+            const uint32_t l0 = length(lane), l1 = length(lane + 32);
+            int r0 = 0, r1 = 0;
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+                const uint32_t a = __shfl_sync(0xffffffffu, l0, j), b = __shfl_sync(0xffffffffu, l1, j);
+                r0 += (a > l0 || (a == l0 && j < lane)) + (b > l0);
+                r1 += (a >= l1) + (b > l1 || (b == l1 && j < lane));
+            }
+            if (l0 && r0 == seq) ctl->seq = lane;
+            if (l1 && r1 == seq) ctl->seq = lane + 32;
+        }
+        __syncthreads();
+        seq = ctl->seq;
+    }
     const int32_t beg = p.cu[seq], end = p.cu[seq + 1];
     if (beg < 0 || end > p.n_rows || beg > end) {
         if (threadIdx.x == 0) atomicOr(p.status, ST_BAD_INDEX);
@@ -882,8 +938,8 @@ __global__ void __launch_bounds__(RK_THREADS, 1) k_rec_chunk(const __grid_consta
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     } else if (threadIdx.x == 0) {
         ctl->abort = 0;
-        for (int i = 0; i < 4 + RK_GROUPS; i++)
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(i < 4 ? &ctl->bar[i] : &ctl->scored[i - 4])) : "memory");
+        for (int i = 0; i < RK_BARS + RK_GROUPS; i++)
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(i < RK_BARS ? &ctl->bar[i] : &ctl->scored[i - RK_BARS])) : "memory");
         asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(&ctl->read)), "r"(RK_GT) : "memory");
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -903,7 +959,7 @@ __global__ void __launch_bounds__(RK_THREADS, 1) k_rec_chunk(const __grid_consta
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(RK_ISSUER_REGS));
         if (threadIdx.x >= RK_ISSUER + 32) return;
-        rk_issue<DELTA>(sm, ctl, beg, end);
+        rk_issue<DELTA>(sm, ctl, beg, end, p.status);
         bar_sync(BAR_END, RK_HAND_N + RK_GROUPS * RK_GT);
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(ctl->tmem), "r"(TM_COLS) : "memory");
