@@ -333,7 +333,8 @@ qkv_status qkv_rec_conv(qkv_engine *eng, int32_t rec_layer, const int32_t *slots
  * of 128 at v + r * v_stride; slices of one fused row are allowed.  g: F32 [rows][rec_n_head], the log
  * of each head's decay (-inf allowed: the state is forgotten; +inf and NaN are not); beta: F32
  * [rows][rec_n_head] for the gated delta rule, NULL for decay alone.  All device; q, k, v 16-byte
- * aligned with strides of whole 16 bytes. */
+ * aligned with strides of whole 16 bytes; none of them (from its first row to its last) overlaps the
+ * output. */
 typedef struct qkv_rec_rows {
     const void  *q, *k, *v;
     int64_t      q_stride, k_stride, v_stride;
@@ -429,7 +430,7 @@ qkv_status qkv_rollback(qkv_engine *eng, int32_t slot, int32_t n_back, void *str
  * eval_batch after a multi-token step, src/qwfn_engine.cpp:3630-3655). */
 qkv_status qkv_rollback_arm(qkv_engine *eng, int32_t slot, int32_t depth);
 
-/* Device pointers of a slot's recurrent state for the (out-of-scope) DeltaNet kernels:
+/* Device pointers of a slot's recurrent state (qkv_rec_conv, qkv_rec_step and qkv_rec_chunk advance it):
  * kind 0 = state [rec_head_dim, rec_head_dim, rec_n_head] F32, kind 1 = conv [conv_hist,
  * conv_channels] F32; which 0 = live state, 1..n_rollback = rollback snapshot which-1.
  * Replaces state::rs_state / rs_conv (src/qwfn_state.h:55-57). */

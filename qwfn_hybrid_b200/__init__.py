@@ -471,6 +471,7 @@ class Engine:
         n = len(slots)
         if len(pos0) != n or len(n_new) != n:
             raise ValueError(f"{n} slots, {len(pos0)} positions, {len(n_new)} lengths")
+        self._on_device(cu, seq, pos, cell, table)
         ctx = self.cfg.n_ctx
         self._check(lib().qkv_batch_map(
             self.handle, _i32_array(slots), _i32_array(pos0), _i32_array(n_new), n, n_rows,
@@ -480,11 +481,17 @@ class Engine:
 
     def append_mapped(self, layer: int, cell, K, V, stream=None) -> None:
         """Quantise F32 rows [n, n_head_kv * head_dim] into the cells of a slot map; -1 skips a row."""
+        self._on_device(cell, K, V)
         n = int(K.shape[0])
         w = n * self.cfg.n_head_kv * self.cfg.head_dim
         self._check(lib().qkv_append_mapped(self.handle, layer, _dense(cell, "torch.int64", n, "cell"),
                                             _dense(K, "torch.float32", w, "K"), _dense(V, "torch.float32", w, "V"), n,
                                             _stream(stream)))
+
+    def _on_device(self, *tensors) -> None:
+        for x in tensors:   # (a host-only engine's device and a host tensor's are both -1)
+            if x is not None and x.get_device() != self.device:
+                raise ValueError(f"tensors of the engine's device {self.device} wanted, got one on {x.device}")
 
     # -- recurrent layers ----------------------------------------------------------------------
     def rec_state(self, rec_layer: int, kind: int = 0, which: int = 0):
@@ -509,6 +516,7 @@ class Engine:
                  stream=None) -> None:
         """Causal convolution of width 4 + silu over ragged rows, heads of the first n_norm channels normalised.
         x: F32 or bf16 rows [n, conv_channels] (a stride between rows is allowed); y: same type, contiguous."""
+        self._on_device(cu, x, w, y)
         kind = str(x.dtype)
         if kind not in ("torch.float32", "torch.bfloat16") or x.dim() != 2 or x.shape[1] != self.cfg.conv_channels:
             raise ValueError(f"x: F32 or bf16 [n, {self.cfg.conv_channels}] wanted, got {x.dtype} {tuple(x.shape)}")
@@ -532,6 +540,7 @@ class Engine:
                  stream=None) -> None:
         """Linear attention with a decay per head (beta: the gated delta rule; None: decay alone), T (1..4) F32
         rows per sequence; the state advances in place."""
+        self._on_device(q, k, v, g, beta, out)
         n = len(slots) * T
         rows = self._rec_rows(q, k, v, g, beta, n, "torch.float32")
         self._check(lib().qkv_rec_step(self.handle, rec_layer, _i32_array(slots), len(slots), ctypes.byref(rows), T, scale,
@@ -540,6 +549,7 @@ class Engine:
 
     def rec_chunk(self, rec_layer: int, slots, cu, q, k, v, g, beta, scale: float, out, stream=None) -> None:
         """The same recurrence over the ragged bf16 rows of prompts (cu: row offsets), in chunks."""
+        self._on_device(cu, q, k, v, g, beta, out)
         n = int(q.shape[0])
         rows = self._rec_rows(q, k, v, g, beta, n, "torch.bfloat16")
         self._check(lib().qkv_rec_chunk(self.handle, rec_layer, _i32_array(slots),

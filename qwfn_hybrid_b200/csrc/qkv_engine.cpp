@@ -1541,8 +1541,18 @@ static qkv_status rec_attn(qkv_engine *eng, int32_t rec_layer, const int32_t *sl
         rows->v_stride < (int64_t)c.rec_n_head * REC_HD || rows->q_stride % per16 || rows->k_stride % per16 || rows->v_stride % per16)
         return fail(eng, QKV_ERR_INVALID, "%s: n_head_k %d of %d heads, null or unaligned pointer, stride below a row or not a multiple of 16 bytes",
                     what, rows ? rows->n_head_k : 0, c.rec_n_head);
+    const int64_t esz = step ? 4 : 2, n_all = step ? (int64_t)n_seq * T : n_rows;
+    const uint8_t *o0 = (const uint8_t *)out, *o1 = o0 + n_all * c.rec_n_head * REC_HD * esz;
+    auto meets_out = [&](const void *x, int64_t stride, int64_t width, int64_t size) {
+        const uint8_t *x0 = (const uint8_t *)x;
+        return x && x0 < o1 && o0 < x0 + ((n_all - 1) * stride + width) * size;
+    };
+    if (meets_out(rows->q, rows->q_stride, (int64_t)rows->n_head_k * REC_HD, esz) ||
+        meets_out(rows->k, rows->k_stride, (int64_t)rows->n_head_k * REC_HD, esz) ||
+        meets_out(rows->v, rows->v_stride, (int64_t)c.rec_n_head * REC_HD, esz) ||
+        meets_out(rows->g, c.rec_n_head, c.rec_n_head, 4) || meets_out(rows->beta, c.rec_n_head, c.rec_n_head, 4))
+        return fail(eng, QKV_ERR_INVALID, "%s: out overlaps an input", what);   // a head's rows may be read after another's are written
     if ((r = use_device(eng)) != QKV_OK) return r;
-    const int64_t esz = step ? 4 : 2;
     for (int32_t base = 0; base < n_seq; base += MAX_SEQ) {
         RecParams p;
         memset(&p, 0, sizeof p);

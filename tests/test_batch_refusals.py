@@ -166,3 +166,38 @@ def test_rec_conv_refusals(qkvlib):
     with pytest.raises(qkvlib.QkvError) as e:
         call()
     assert e.value.status == qkvlib.ERR_UNSUPPORTED
+
+
+def test_rec_output_over_an_input_is_refused(qkvlib):
+    eng = host_engine(qkvlib)
+    for name in ("q", "k", "v", "g", "beta"):
+        buf = torch.zeros(6 * 1024)
+        out = buf[:2 * 512].view(2, 4, 128)                    # the last values of out and the first of the input
+        width = {"q": 256, "k": 256, "v": 512, "g": 4, "beta": 4}[name]
+        at = 2 * 512
+        for start, status in ((at - 4, "INVALID"), (at, "UNSUPPORTED")):
+            with pytest.raises(qkvlib.QkvError) as e:
+                step(eng, out=out, **{name: buf[start:start + 2 * width].view(2, width)})
+            assert e.value.status == getattr(qkvlib, "ERR_" + status), (name, start)
+    r = rows(6, dtype=torch.bfloat16)
+    with pytest.raises(qkvlib.QkvError) as e:                     # out in the place of v
+        v = torch.zeros(6, 512, dtype=torch.bfloat16)
+        eng.rec_chunk(0, [0, 1], CU, r["q"], r["k"], v, r["g"], r["beta"], 1.0, v.view(6, 4, 128))
+    assert e.value.status == qkvlib.ERR_INVALID
+
+
+def test_tensors_of_another_device_are_refused(qkvlib):
+    eng = host_engine(qkvlib)
+    eng.device = 0                                                 # host tensors for a device's engine: nothing is called
+    i32 = torch.zeros(3, dtype=torch.int32)
+    r, b = rows(), rows(6, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="device"):
+        eng.batch_map([0], [0], [1], 1, i32)
+    with pytest.raises(ValueError, match="device"):
+        eng.append_mapped(0, torch.zeros(2, dtype=torch.int64), torch.zeros(2, 512), torch.zeros(2, 512))
+    with pytest.raises(ValueError, match="device"):
+        step(eng, **r)
+    with pytest.raises(ValueError, match="device"):
+        eng.rec_chunk(0, [0, 1], CU, b["q"], b["k"], b["v"], b["g"], None, 1.0, torch.zeros(6, 4, 128, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="device"):
+        eng.rec_conv(0, [0, 1], CU, torch.zeros(6, 1024), torch.zeros(1024, 4), torch.zeros(6, 1024))

@@ -119,8 +119,9 @@ def test_step_forgets_at_minus_infinity(cuda, qkvlib):
 
 # A chunk of 64 tokens: state and sums in 32 bits, products of operands split so that a factor is off by at most
 # 2^-22 of its row's largest value; under 64 half steps of 2^-24 of the sums over absolute values for
-# each 64 tokens and the ones that the first state carries.  The output meets three operands rounded to 11
-# bits (the state, the scores, u), 2^-11 each of those sums, and its own rounding, 2^-8 of the value.
+# each 64 tokens and the ones that the first state carries.  The output meets three operands cut to 16
+# bits (the state, the scores, u), under 2^-15 each of those sums (2^-11 is allowed), and its own rounding, 2^-8 of the
+# value.
 CHUNK = 64 * 2.0 ** -24
 
 
