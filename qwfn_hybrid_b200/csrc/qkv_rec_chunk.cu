@@ -14,10 +14,10 @@
 // there (lane = value row: no shuffles, no shared memory); B is k, q, T and P in shared memory as they are.  Per
 // chunk: X = S k^T, U = R T^T, O = S q^T, S += (w U) k (k as an MN-major operand, the same bytes), O += U P^T.  A warp of
 // its own issues the products, so that no other waits for the tensor cores to take one; S q^T goes behind what the
-// chain waits for (beside X, as one product of 128 columns, a 16K prompt takes 4% longer).  The chain reads a chunk's O while
+// chain waits for (beside X, as one product of 128 columns, a 16K prompt took 4% longer).  The chain reads a chunk's O while
 // the next chunk's X is made, and stores it while that chunk's part of S is made.
 //
-// Where the sequences are more than two, the CTAs take the longest first (24 prompts of 24001 rows: 656 against 690 us).
+// Where the sequences are more than two, the CTAs take the longest first (24 prompts of 24001 rows: 5% less).
 //
 // Precision.  k and q are exact in bf16, so S, w U and U enter as sums of bf16 terms (three: 24 bits; two for what
 // only the rounded output sees, as P; truncated terms, which need no conversion: three of them are the value), and T
@@ -30,13 +30,16 @@
 // tokens; such chunks (and those with g > 0, a growing state, which could leave the range of what is scaled) are
 // flagged by the producers and run token by token from global memory.
 //
-// What bounds it: neither bytes nor the tensor cores (60 products of 64 cycles a chunk) but the chain's latency -- four
-// round trips from registers through tensor memory and a product a chunk -- and, beside it on the same
-// schedulers, the producers'.  A chunk takes 5.25 us (delta rule, 16384 tokens: 1345 us) or 3.7 us; alone the
-// producers take 4.1 us (delta rule), and a shorter way to T (blocks of 8, fewer barriers, shorter chains of products)
-// changed nothing.  A kernel of the same split on mma.sync, 64 value rows per CTA with S as the accumulator that is the
-// next product's A operand, took 5.9 us per chunk and half a head, 1.6 to 1.75 times as long where the heads fill the
-// GPU (24 prompts of 24001 rows: 1097 against 656 us).
+// What bounds it: neither bytes nor the tensor cores (56 products of 32 or 64 cycles a chunk) but the chain's latency -- four
+// round trips from registers through tensor memory and a product a chunk -- and, beside it on the same schedulers, the
+// producers'.  A chunk takes 5.0 us (delta rule, 16384 tokens: 1280 us) or 3.5 us (decay alone).  From about 100
+// CTAs on it takes longer, 5.3 to 7.6 us: the three roles' loops are more instructions than an SM keeps, and the SMs of a group
+// fetch them from one cache (at 148 CTAs warps waited 3.5 cycles per instruction for instructions, at 32 CTAs 0.4).  So the
+// code is kept short where time allows: one body for the rows of k and of q, loops over tiles of T and over the terms of a
+// product (24 prompts of 24001 rows, 32 heads: 656 -> 556 us); with all products in loops 148 equal CTAs take 6.4 us, but few of
+// them 5.4.  Not kept: a long sequence in three parts by clusters of three CTAs (the state is linear in the one it starts
+// from) took 1160 instead of 1310 us and, through its registers, made all other sizes 3 to 7% slower; a kernel of the same split on
+// mma.sync, 64 value rows per CTA, took 5.9 us per chunk and half a head.
 #include "qkv_internal.h"
 
 #include <cuda_bf16.h>
@@ -431,46 +434,30 @@ __device__ __forceinline__ void rk_produce(const RecParams &p, uint8_t *sm, RkCt
         {   // a row per thread: warps 0, 1 rows of k k^T (-A; delta rule), warps 2, 3 of q k^T (P)
             const uint32_t tg = tm + TM_G + ((uint32_t)(32 * wid) << 16);
             const int i = tid & 63;
-            float x[32];
-            if (wid == 0) {
-                tm_ld32(tg, x);
-                tm_wait_ld(x);
-                if (DELTA) {
-                    bad |= rk_not_finite(x);
-                    rk_decay<true>(x, cf, i, 0, -bs[i], true);
-                    rk_store_a(As, i, 0, x);
-                }
-            } else if (wid == 1) {
-                tm_ld32(tg, x);
-                tm_wait_ld(x);
-                if (DELTA) {
-                    rk_decay<false>(x, cf, i, 0, -bs[i], true);
-                    rk_store_a(As, i, 0, x);
-                    tm_ld32(tg + 32, x);
+            const bool of_k = wid < 2;
+            if (DELTA || !of_k) {
+                const float f = of_k ? -bs[i] : 1.0f;
+#pragma unroll 1
+                for (int j = 0; j <= (wid & 1); j++) {   // 32 tokens of the row: below the diagonal block, then that
+                    float x[32];
+                    tm_ld32(tg + 32 * j, x);
                     tm_wait_ld(x);
-                    bad |= rk_not_finite(x);
-                    rk_decay<true>(x, cf, i, 32, -bs[i], true);
-                    rk_store_a(As, i, 2, x);
-                }
-            } else {
-                tm_ld32(tg, x);
-                tm_wait_ld(x);
-                if (wid == 3) {
-                    rk_decay<false>(x, cf, i, 0, 1.0f, false);
-                    rk_store_p(sg, i, 0, x);
-                    tm_ld32(tg + 32, x);
-                    tm_wait_ld(x);
-                }
-                bad |= rk_not_finite(x);
-                rk_decay<true>(x, cf, i, 32 * (wid - 2), 1.0f, false);
-                rk_store_p(sg, i, wid - 2, x);
-                if (wid == 2) {   // nothing right of the diagonal blocks
-#pragma unroll
-                    for (int c = 4; c < 8; c++) {
-                        const int off = i * 128 + ((c ^ (i & 7)) << 4);
-                        *reinterpret_cast<uint4 *>(sg + RK_PH + off) = make_uint4(0, 0, 0, 0);
-                        *reinterpret_cast<uint4 *>(sg + RK_PM + off) = make_uint4(0, 0, 0, 0);
+                    if (j == (wid & 1)) {
+                        bad |= rk_not_finite(x);
+                        rk_decay<true>(x, cf, i, 32 * j, f, of_k);
+                    } else {
+                        rk_decay<false>(x, cf, i, 0, f, of_k);
                     }
+                    if (of_k) rk_store_a(As, i, 2 * j, x);
+                    else rk_store_p(sg, i, j, x);
+                }
+            }
+            if (wid == 2) {   // nothing right of the diagonal blocks
+#pragma unroll
+                for (int c = 4; c < 8; c++) {
+                    const int off = i * 128 + ((c ^ (i & 7)) << 4);
+                    *reinterpret_cast<uint4 *>(sg + RK_PH + off) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4 *>(sg + RK_PM + off) = make_uint4(0, 0, 0, 0);
                 }
             }
             tc_fence_before();
@@ -479,53 +466,74 @@ __device__ __forceinline__ void rk_produce(const RecParams &p, uint8_t *sm, RkCt
         if (bad) cf[CF_N * RK_C + 1] = 1.0f;
         if (DELTA) {
             bar_sync(BAR_PROD + grp, RK_GT);
-            // T in place of A.  The four 16 x 16 tiles on the diagonal by forward substitution,
-            // x_i = [i = column] - sum_{j < i} A_ij x_j, one per warp, a column per lane;
-            if (lane < 16) {
+            // T in place of A.  The 16 x 16 tiles on the diagonal, one per warp: their 8 x 8 blocks on the diagonal by
+            // forward substitution, x_i = [i = column] - sum_{j < i} A_ij x_j, a column per lane, then the block below,
+            // -T_11 A_10 T_00, two of its values per lane (A is held negated);
+            {
                 float *a = As + (wid * (wid + 1) / 2 + wid) * RK_TILE;
-                float y[16];
+                if (lane < 16) {
+                    float *d = a + (lane >> 3) * (8 * RK_PITCH + 8), y[8];
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    float s0 = i == lane ? 1.0f : 0.0f, s1 = 0.0f;
+                    for (int i = 0; i < 8; i++) {
+                        float s0 = i == (lane & 7) ? 1.0f : 0.0f, s1 = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < i; j += 4) {
-                        const float4 u = *reinterpret_cast<const float4 *>(a + i * RK_PITCH + j);
-                        s0 = fmaf(u.x, y[j], s0);
-                        if (j + 1 < i) s1 = fmaf(u.y, y[j + 1], s1);
-                        if (j + 2 < i) s0 = fmaf(u.z, y[j + 2], s0);
-                        if (j + 3 < i) s1 = fmaf(u.w, y[j + 3], s1);
+                        for (int j = 0; j < i; j += 4) {
+                            const float4 u = *reinterpret_cast<const float4 *>(d + i * RK_PITCH + j);
+                            s0 = fmaf(u.x, y[j], s0);
+                            if (j + 1 < i) s1 = fmaf(u.y, y[j + 1], s1);
+                            if (j + 2 < i) s0 = fmaf(u.z, y[j + 2], s0);
+                            if (j + 3 < i) s1 = fmaf(u.w, y[j + 3], s1);
+                        }
+                        y[i] = s0 + s1;
                     }
-                    y[i] = s0 + s1;
-                }
-                __syncwarp(0xffffu);
+                    __syncwarp(0xffffu);
 #pragma unroll
-                for (int i = 0; i < 16; i++) a[i * RK_PITCH + lane] = y[i];
+                    for (int i = 0; i < 8; i++) d[i * RK_PITCH + (lane & 7)] = y[i];
+                }
+                __syncwarp();
+                float *lo = a + (8 + g) * RK_PITCH, *x = a + 2 * t;   // a row of the block below, two columns
+#pragma unroll
+                for (int s = 0; s < 2; s++) {   // A_10 T_00 in A_10's place, then T_11 times that
+                    const float *l = lo + 8 * s, *r = x + (s ? 8 * RK_PITCH : 0);
+                    float v0 = 0.0f, v1 = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 8; k += 4) {
+                        const float4 u = *reinterpret_cast<const float4 *>(l + k);
+                        const float2 r0 = *reinterpret_cast<const float2 *>(r + k * RK_PITCH), r1 = *reinterpret_cast<const float2 *>(r + (k + 1) * RK_PITCH);
+                        const float2 r2 = *reinterpret_cast<const float2 *>(r + (k + 2) * RK_PITCH), r3 = *reinterpret_cast<const float2 *>(r + (k + 3) * RK_PITCH);
+                        v0 = fmaf(u.w, r3.x, fmaf(u.z, r2.x, fmaf(u.y, r1.x, fmaf(u.x, r0.x, v0))));
+                        v1 = fmaf(u.w, r3.y, fmaf(u.z, r2.y, fmaf(u.y, r1.y, fmaf(u.x, r0.y, v1))));
+                    }
+                    __syncwarp();
+                    *reinterpret_cast<float2 *>(lo + 2 * t) = make_float2(v0, v1);
+                    __syncwarp();
+                }
             }
             bar_sync(BAR_PROD + grp, RK_GT);
-            // the tiles beside them, T_10 = -T_11 A_10 T_00 (tiles 1, 0; 3, 2);
+            // the tiles beside them, T_10 = -T_11 A_10 T_00 (tiles 1, 0; 3, 2), A_10 T_00 first in A_10's place;
             if (wid < 2) {
                 float *lo = As + (wid ? 8 : 1) * RK_TILE;                    // tile (1, 0) or (3, 2)
-                float u[2][4] = {}, w[2][4] = {};
-                rk_tile(u, lo, As + (wid ? 5 : 0) * RK_TILE, g, t);
-                __syncwarp();
-                rk_tile_store(lo, u, g, t);
-                __syncwarp();
-                rk_tile(w, As + (wid ? 9 : 2) * RK_TILE, lo, g, t);
-                __syncwarp();
-                rk_tile_store(lo, w, g, t);
+#pragma unroll 1
+                for (int k = 0; k < 2; k++) {
+                    float u[2][4] = {};
+                    rk_tile(u, k ? lo + RK_TILE : lo, k ? lo : As + (wid ? 5 : 0) * RK_TILE, g, t);
+                    __syncwarp();
+                    rk_tile_store(lo, u, g, t);
+                    __syncwarp();
+                }
             }
             bar_sync(BAR_PROD + grp, RK_GT);
             {   // then the lower left 32 x 32: -T_1 A_10 T_0, a tile (a, b) of it per warp
                 const int a = wid >> 1, b = wid & 1;
                 float *lo = As + (a ? 6 : 3) * RK_TILE;                      // tiles (2 + a, 0) and (2 + a, 1)
                 float u[2][4] = {}, w[2][4] = {};
-                if (b == 0) rk_tile(u, lo, As, g, t);                        // M_ab = -sum_k A_(2+a)k T_kb, in A's place
-                rk_tile(u, lo + RK_TILE, As + (b ? 2 : 1) * RK_TILE, g, t);
+#pragma unroll 1
+                for (int k = b; k < 2; k++) rk_tile(u, lo + k * RK_TILE, As + k * (1 + b) * RK_TILE, g, t);   // M_ab = -sum_k A_(2+a)k T_kb, in A's place
                 bar_sync(BAR_PROD + grp, RK_GT);
                 rk_tile_store(lo + b * RK_TILE, u, g, t);
                 bar_sync(BAR_PROD + grp, RK_GT);
-                rk_tile(w, As + (a ? 8 : 5) * RK_TILE, As + (3 + b) * RK_TILE, g, t);
-                if (a == 1) rk_tile(w, As + 9 * RK_TILE, As + (6 + b) * RK_TILE, g, t);
+#pragma unroll 1
+                for (int k = 0; k <= a; k++) rk_tile(w, As + (5 + 3 * a + k) * RK_TILE, As + (3 + b + 3 * k) * RK_TILE, g, t);
                 bar_sync(BAR_PROD + grp, RK_GT);
                 rk_tile_store(lo + b * RK_TILE, w, g, t);
             }
@@ -605,7 +613,7 @@ __device__ __forceinline__ void rk_issue(uint8_t *sm, RkCtl *ctl, int32_t beg, i
         bar_sync(BAR_HAND, RK_HAND_N);
         tc_fence_after();
         auto times_s = [&](uint32_t d, uint64_t b, int terms) {   // S times 64 rows of k or q
-#pragma unroll
+#pragma unroll (DELTA ? 1 : 3)
             for (int term = 0; term < terms; term++)
 #pragma unroll
                 for (int kk = 0; kk < 8; kk++)
@@ -646,7 +654,7 @@ __device__ __forceinline__ void rk_issue(uint8_t *sm, RkCtl *ctl, int32_t beg, i
         tc_fence_after();
         rk_wait(&ctl->bar[4], parity, ctl, status);   // the last reader of S's terms, which the new part replaces
         if (one) {   // the new part of S
-#pragma unroll
+#pragma unroll (DELTA ? 1 : 3)
             for (int term = 0; term < 3; term++)
 #pragma unroll
                 for (int ks = 0; ks < 4; ks++)
@@ -657,7 +665,7 @@ __device__ __forceinline__ void rk_issue(uint8_t *sm, RkCtl *ctl, int32_t beg, i
         bar_sync(BAR_HAND_U, RK_HAND_N);
         tc_fence_after();
         if (one) {   // O's part from this chunk's tokens
-#pragma unroll
+#pragma unroll (DELTA ? 1 : 3)
             for (int term = 0; term < 3; term++)
 #pragma unroll
                 for (int ks = 0; ks < 4; ks++)
@@ -741,11 +749,20 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
         if (out_t0 < 0) return;
         __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out) + (int64_t)(out_t0 + 32 * half) * out_row + (int64_t)h * REC_HD + row;
         const int n = end - out_t0 - 32 * half;
+        if (!DELTA && n >= 32) {   // (4% there; with the delta rule the longer code costs as much)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            if (2 * i < n) *reinterpret_cast<uint16_t *>(out) = (uint16_t)ow[i];
-            if (2 * i + 1 < n) *reinterpret_cast<uint16_t *>(out + out_row) = (uint16_t)(ow[i] >> 16);
-            out += 2 * out_row;
+            for (int i = 0; i < 16; i++) {
+                *reinterpret_cast<uint16_t *>(out) = (uint16_t)ow[i];
+                *reinterpret_cast<uint16_t *>(out + out_row) = (uint16_t)(ow[i] >> 16);
+                out += 2 * out_row;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                if (2 * i < n) *reinterpret_cast<uint16_t *>(out) = (uint16_t)ow[i];
+                if (2 * i + 1 < n) *reinterpret_cast<uint16_t *>(out + out_row) = (uint16_t)(ow[i] >> 16);
+                out += 2 * out_row;
+            }
         }
         out_t0 = -1;
     };

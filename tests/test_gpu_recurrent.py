@@ -252,6 +252,89 @@ def test_chunk_is_the_same_twice_and_continues(cuda, qkvlib):
     assert torch.equal(outs[0], outs[1]) and torch.equal(states[0], states[1])
 
 
+def long_reference(S, q, k, v, g, beta, scale):
+    """One long sequence in 64 bits: out, the last state, and the largest norm of a head's state on the way."""
+    S, q, k, v, e, beta = S.double(), heads(q).double(), heads(k).double(), heads(v).double(), torch.exp(g.double()), beta.double()
+    n = S.shape[0] // q.shape[1]
+    q, k = q.repeat_interleave(n, 1), k.repeat_interleave(n, 1)
+    out, most = torch.empty_like(v), S.flatten(1).norm(dim=1)
+    for t in range(v.shape[0]):
+        S = S * e[t, :, None, None]
+        u = beta[t, :, None] * (v[t] - (S * k[t, :, None, :]).sum(-1))
+        S = S + u[:, :, None] * k[t, :, None, :]
+        out[t] = scale * (S * q[t, :, None, :]).sum(-1)
+        most = torch.maximum(most, S.flatten(1).norm(dim=1))
+    return out, S, most
+
+
+def in_pieces(eng, slots, lengths, q, k, v, g, beta, out, piece=1024):
+    """The same sequences, `piece` rows to a call."""
+    at = 0
+    for s, n in zip(slots, lengths):
+        for a in range(at, at + n, piece):
+            r = slice(a, min(a + piece, at + n))
+            eng.rec_chunk(0, [s], offsets([r.stop - r.start]), q[r], k[r], v[r], g[r], beta[r], SCALE, out[r])
+        at += n
+
+
+@pytest.mark.parametrize("lengths,H,Hk,decay", [([2048], 4, 2, 1e-3), ([2049, 4161, 2500], 3, 3, 1e-3), ([3000, 0, 4000], 2, 1, 0.3),
+                                                ([5000, 1500, 77], 2, 2, 1e-5)])
+def test_chunk_long_sequences(cuda, qkvlib, lengths, H, Hk, decay):
+    """Many chunks, in one call and in calls of 1024 rows."""
+    n, rows = len(lengths), sum(lengths)
+    engs = [rec_engine(qkvlib, H, Hk, n_slots=n, layers=1) for _ in range(2)]
+    S0 = fill(engs[0], 61, scale=1.0)
+    fill(engs[1], 61, scale=1.0)
+    q, k, v, g, beta = inputs(62, rows, H, Hk, torch.bfloat16, decay=decay)
+    out, other = (torch.full((rows + 1, H, HD), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    engs[0].rec_chunk(0, list(range(n)), offsets(lengths), q, k, v, g, beta, SCALE, out)
+    in_pieces(engs[1], range(n), lengths, q, k, v, g, beta, other)
+    assert bool((out[rows] == 7.0).all())
+    S1, S2, at = engs[0].rec_state(0), engs[1].rec_state(0), 0
+    for i, m in enumerate(lengths):
+        r = slice(at, at + m)
+        at += m
+        ref, S, most = long_reference(S0[i], q[r], k[r], v[r], g[r], beta[r], SCALE)
+        # keys of length one, beta below one and no growth: no token lengthens an error, so each chunk adds its own, under
+        # 64 half steps of 2^-24 of the state's norm; the output is rounded once, 2^-8, its operands by less than a
+        # tenth of that
+        for what, got in (("whole", S1[i]), ("pieces", S2[i])):
+            err = (got.double() - S).flatten(1).norm(dim=1)
+            assert bool((err <= ((m + 63) // 64 + 1) * CHUNK * most).all()), f"{what}, state of sequence {i}: {float((err / most).max()):.2e}"
+        if m:
+            for what, got in (("whole", out[r]), ("pieces", other[r])):
+                rel = ((got.double() - ref).flatten().norm() / ref.flatten().norm()).item()
+                assert rel <= 1.1 * 2.0 ** -8, f"{what}, out of sequence {i}: {rel:.2e}"
+
+
+@pytest.mark.parametrize("what", ["nan", "inf in k", "nan in q", "grows", "long keys"])
+@pytest.mark.parametrize("at", [100, 1000, 2000])
+def test_chunk_long_sequences_out_of_range(cuda, qkvlib, what, at):
+    """A value early, in the middle and late that is not finite, or a state that grows: as in calls of 1024 rows."""
+    m, H = 2400, 2
+    engs = [rec_engine(qkvlib, H, 1, n_slots=1, layers=1) for _ in range(2)]
+    for e in engs:
+        fill(e, 63)
+    q, k, v, g, beta = inputs(64, m, H, 1, torch.bfloat16, decay=1e-2)
+    if what == "nan":
+        v[at, 5] = float("nan")
+    elif what == "inf in k":
+        k[at, 3] = float("inf")
+    elif what == "nan in q":
+        q[at, 3] = float("nan")
+    elif what == "grows":
+        g[at, 1] = 0.25
+    else:
+        k[at:at + 200] *= 1.75
+    outs = [torch.zeros(m, H, HD, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    engs[0].rec_chunk(0, [0], offsets([m]), q, k, v, g, beta, SCALE, outs[0])
+    in_pieces(engs[1], [0], [m], q, k, v, g, beta, outs[1])
+    for a, b, tol in ((engs[0].rec_state(0), engs[1].rec_state(0), 2 * 39 * CHUNK), (*outs, 2.2 * 2.0 ** -8)):
+        assert torch.equal(a.isfinite(), b.isfinite())
+        a, b = (x.double().nan_to_num(0.0, 0.0, 0.0) for x in (a, b))
+        assert float((a - b).norm()) <= tol * float(b.norm())
+
+
 def test_chunk_bad_offsets_are_reported(cuda, qkvlib):
     eng = rec_engine(qkvlib, 2, 1, n_slots=3)
     S0 = fill(eng, 23)
