@@ -129,11 +129,11 @@ def lib() -> ctypes.CDLL:
         "qkv_static_status": [P, pI32],
         "qkv_debug_decode_wait": [P, I64, I32],
         "qkv_attn_prefill_qsa": [P, I32, I32, I32, P, P, I32, F32, P, P, P, P],
-        "qkv_batch_map": [P, pI32, pI32, pI32, I32, I32, P, P, P, P, P, P],
+        "qkv_batch_map": [P, P, P, P, I32, I32, P, P, P, P, P, P],
         "qkv_append_mapped": [P, I32, P, P, P, I32, P],
-        "qkv_rec_conv": [P, I32, pI32, P, I32, I32, P, I64, P, I32, I32, F32, P, I32, P],
-        "qkv_rec_step": [P, I32, pI32, I32, ctypes.POINTER(QkvRecRows), I32, F32, P, I32, P],
-        "qkv_rec_chunk": [P, I32, pI32, P, I32, ctypes.POINTER(QkvRecRows), I32, F32, P, P],
+        "qkv_rec_conv": [P, I32, P, P, I32, I32, P, I64, P, I32, I32, F32, P, I32, P],
+        "qkv_rec_step": [P, I32, P, I32, ctypes.POINTER(QkvRecRows), I32, F32, P, I32, P],
+        "qkv_rec_chunk": [P, I32, P, P, I32, ctypes.POINTER(QkvRecRows), I32, F32, P, P],
         "qkv_debug_check_q8_scale": [ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64)],
     }
     for name, args in sig.items():
@@ -157,6 +157,14 @@ def _i32_array(values) -> ctypes.Array:
         return (ctypes.c_int32 * max(1, n))(*[int(v) for v in values])
 
 
+def _i32s(values) -> array.array:
+    """int32 values whose buffer_info()[0] is passed as a pointer while the array lives (cheaper than a ctypes array)."""
+    try:
+        return array.array("i", values)
+    except TypeError:
+        return array.array("i", [int(v) for v in values])
+
+
 def _ptr(x) -> int | None:
     """Device pointer of a torch tensor (contiguous) or a raw integer address; None -> NULL."""
     if x is None:
@@ -168,9 +176,18 @@ def _ptr(x) -> int | None:
     return x.data_ptr()
 
 
+class _Names(dict):
+    def __missing__(self, dtype):
+        self[dtype] = name = str(dtype)
+        return name
+
+
+_names = _Names()   # of dtypes: str(dtype) costs several times a look-up
+
+
 def _rows(x, dtype: str):
     """Pointer, row stride (elements) and row width of a tensor of rows [n, ...] whose rows are contiguous."""
-    if str(x.dtype) != dtype:
+    if _names[x.dtype] != dtype:
         raise ValueError(f"rows of {dtype} wanted, got {x.dtype}")
     shape, strides = x.shape, x.stride()
     want = 1
@@ -185,7 +202,7 @@ def _dense(x, dtype: str, n: int, what: str):
     """Pointer of a contiguous tensor of dtype with at least n elements; None -> NULL."""
     if x is None:
         return None
-    if str(x.dtype) != dtype or not x.is_contiguous() or x.numel() < n:
+    if _names[x.dtype] != dtype or not x.is_contiguous() or x.numel() < n:
         raise ValueError(f"{what}: contiguous {dtype} of at least {n} elements wanted, got {x.dtype} {tuple(x.shape)}")
     return x.data_ptr()
 
@@ -473,8 +490,9 @@ class Engine:
             raise ValueError(f"{n} slots, {len(pos0)} positions, {len(n_new)} lengths")
         self._on_device(cu, seq, pos, cell, table)
         ctx = self.cfg.n_ctx
+        s, p, m = _i32s(slots), _i32s(pos0), _i32s(n_new)
         self._check(lib().qkv_batch_map(
-            self.handle, _i32_array(slots), _i32_array(pos0), _i32_array(n_new), n, n_rows,
+            self.handle, s.buffer_info()[0], p.buffer_info()[0], m.buffer_info()[0], n, n_rows,
             _dense(cu, "torch.int32", n + 1, "cu"), _dense(seq, "torch.int32", n_rows, "seq"),
             _dense(pos, "torch.int32", n_rows, "pos"), _dense(cell, "torch.int64", n_rows, "cell"),
             _dense(table, "torch.int32", n * ((ctx + 255) // 256), "table"), _stream(stream) if self.device >= 0 else None))
@@ -517,13 +535,14 @@ class Engine:
         """Causal convolution of width 4 + silu over ragged rows, heads of the first n_norm channels normalised.
         x: F32 or bf16 rows [n, conv_channels] (a stride between rows is allowed); y: same type, contiguous."""
         self._on_device(cu, x, w, y)
-        kind = str(x.dtype)
+        kind = _names[x.dtype]
         if kind not in ("torch.float32", "torch.bfloat16") or x.dim() != 2 or x.shape[1] != self.cfg.conv_channels:
             raise ValueError(f"x: F32 or bf16 [n, {self.cfg.conv_channels}] wanted, got {x.dtype} {tuple(x.shape)}")
         n = int(x.shape[0])
         ptr, stride, _ = _rows(x, kind)
+        s = _i32s(slots)
         self._check(lib().qkv_rec_conv(
-            self.handle, rec_layer, _i32_array(slots), _dense(cu, "torch.int32", len(slots) + 1, "cu"), len(slots),
+            self.handle, rec_layer, s.buffer_info()[0], _dense(cu, "torch.int32", len(slots) + 1, "cu"), len(slots),
             F32 if kind == "torch.float32" else BF16, ptr, stride,
             _dense(w, "torch.float32", 4 * self.cfg.conv_channels, "w"), n, n_norm, eps,
             _dense(y, kind, n * self.cfg.conv_channels, "y"), int(save), _stream(stream)))
@@ -543,7 +562,8 @@ class Engine:
         self._on_device(q, k, v, g, beta, out)
         n = len(slots) * T
         rows = self._rec_rows(q, k, v, g, beta, n, "torch.float32")
-        self._check(lib().qkv_rec_step(self.handle, rec_layer, _i32_array(slots), len(slots), ctypes.byref(rows), T, scale,
+        s = _i32s(slots)
+        self._check(lib().qkv_rec_step(self.handle, rec_layer, s.buffer_info()[0], len(slots), ctypes.byref(rows), T, scale,
                                        _dense(out, "torch.float32", n * self.cfg.rec_n_head * self.cfg.rec_head_dim, "out"),
                                        int(save), _stream(stream)))
 
@@ -552,7 +572,8 @@ class Engine:
         self._on_device(cu, q, k, v, g, beta, out)
         n = int(q.shape[0])
         rows = self._rec_rows(q, k, v, g, beta, n, "torch.bfloat16")
-        self._check(lib().qkv_rec_chunk(self.handle, rec_layer, _i32_array(slots),
+        s = _i32s(slots)
+        self._check(lib().qkv_rec_chunk(self.handle, rec_layer, s.buffer_info()[0],
                                         _dense(cu, "torch.int32", len(slots) + 1, "cu"), len(slots), ctypes.byref(rows), n, scale,
                                         _dense(out, "torch.bfloat16", n * self.cfg.rec_n_head * self.cfg.rec_head_dim, "out"),
                                         _stream(stream)))
