@@ -448,3 +448,44 @@ def test_captured_and_replayed(cuda, qkvlib):
         graph.replay()
         assert torch.equal(out, want[i])
     assert torch.equal(engs[0].rec_state(0), engs[1].rec_state(0))
+
+
+def test_layers_on_two_streams_at_once(cuda, qkvlib):
+    """Calls share nothing but the engine: two layers' prompts and steps on two streams, eager beside a replayed graph."""
+    H, Hk, lengths = 4, 2, [700, 65, 1300]
+    n, rows = len(lengths), sum(lengths)
+    eng, other = (rec_engine(qkvlib, H, Hk, n_slots=n) for _ in range(2))
+    cu, ch = offsets(lengths), (2 * Hk + H) * HD
+    gen = torch.Generator().manual_seed(71)
+    x = [torch.randn(rows, ch, generator=gen).bfloat16().cuda() for _ in range(2)]
+    w = torch.randn(ch, 4, generator=gen).cuda()
+    g, beta = -torch.rand(rows, H, generator=gen).cuda(), torch.rand(rows, H, generator=gen).cuda()
+    y, out = [torch.empty_like(x[0]) for _ in range(2)], [torch.empty(rows, H, HD, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+
+    def prompt(e, layer, y, out):
+        e.rec_conv(layer, list(range(n)), cu, x[layer], w, y, n_norm=2 * Hk * HD)
+        e.rec_chunk(layer, list(range(n)), cu, y[:, :Hk * HD], y[:, Hk * HD:2 * Hk * HD], y[:, 2 * Hk * HD:], g, beta, SCALE, out)
+
+    want = []
+    for layer in range(2):
+        for e in (eng, other):
+            fill(e, 72 + layer, layer=layer)
+            fill(e, 74 + layer, kind=1, layer=layer)
+        prompt(other, layer, y[0], out[0])
+        prompt(other, layer, y[0], out[0])
+        want.append(out[0].clone())
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        prompt(eng, 0, y[0], out[0])
+    torch.cuda.synchronize()
+    for _ in range(2):
+        with torch.cuda.stream(streams[0]):
+            graph.replay()
+        with torch.cuda.stream(streams[1]):
+            prompt(eng, 1, y[1], out[1])
+    torch.cuda.synchronize()
+    for layer in range(2):
+        assert torch.equal(out[layer], want[layer])
+        for kind in range(2):
+            assert torch.equal(eng.rec_state(layer, kind), other.rec_state(layer, kind))
