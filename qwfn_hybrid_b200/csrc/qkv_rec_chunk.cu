@@ -650,7 +650,7 @@ __device__ __forceinline__ void rk_issue(uint8_t *sm, RkCtl *ctl, int32_t beg, i
             }
             __syncwarp();
         }
-        bar_sync(BAR_HAND, RK_HAND_N);
+        bar_sync(DELTA ? BAR_HAND : BAR_CHAIN, RK_HAND_N);
         tc_fence_after();
         rk_wait(&ctl->bar[4], parity, ctl, status);   // the last reader of S's terms, which the new part replaces
         if (one) {   // the new part of S
@@ -878,7 +878,9 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
             tm_st8(tl + TM_X + 32 * half + 16 + 8 * b, w1);
             tm_st8(tl + TM_S2 + 16 * half + 8 * b, w2);
         }
-        hand_over(BAR_HAND);
+        // (With the delta rule two waits for products lie between a chunk's hand-overs on one barrier.  Without it nothing does: a
+        // fast warp's second arrival must not stand for a slow one's first.)
+        hand_over(DELTA ? BAR_HAND : BAR_CHAIN);
         // U in two terms for the output
 #pragma unroll
         for (int b = 0; b < 2; b++) {
