@@ -86,10 +86,15 @@ enum { BAR_FULL = 1, BAR_EMPTY = BAR_FULL + RK_STAGES, BAR_PROD = BAR_EMPTY + RK
 static_assert(BAR_END < 16, "named barriers");
 constexpr int RK_FULL_N = RK_GT + RK_CHAIN + 32, RK_EMPTY_N = RK_GT + RK_CHAIN, RK_HAND_N = RK_CHAIN + 32;
 // tensor memory columns.  S: half h (keys 64 h ..) has its leading and middle terms at 64 h, 64 h + 32, its last at
-// 128 + 32 h; the new part of S comes back over the first 128 (each thread reads and writes its own 64).  X: tokens
-// 32 h .. at 32 h; R's two terms replace what its thread has read, then two of w U's; the third takes the place
-// of S's last, as U's leading term does.  O's second part replaces U.  Then the producers' scores, and U's second term.
-constexpr uint32_t TM_S = 0, TM_S2 = 128, TM_X = 192, TM_O1 = 256, TM_U = 320, TM_U2 = 384, TM_G = 416, TM_UM = 480, TM_COLS = 512;
+// TM_S2 or (h = 1) TM_U2; the new part of S comes back over the first 128 (each thread reads and writes its own 64).  X:
+// tokens 32 h .. at 32 h; R's two terms replace what its thread has read, then two of w U's; the third takes the place
+// of S's last (h = 0).  O's second part replaces U.  Then the producers' scores, and U's terms for O.
+// What lets a region be written again, chunk c's last reader of it in brackets: TM_S and w U's terms, bar[2] of c (S's
+// product, behind bar[4] in the issuer); S's last terms [X's product], bar[0] of c, and at TM_U2 the thread that writes them is
+// the one that read U there; R [U's product], bar[1]; U's two terms for O (TM_UL, TM_UM) [O's second part, which c + 1's S
+// does not wait for], bar[3] of c, which each thread waits for before it hands over R (delta rule) or starts c + 1; O and U, the hand-over of
+// R (delta rule) or of S, behind every thread's read of them.
+constexpr uint32_t TM_S = 0, TM_S2 = 128, TM_UL = 160, TM_X = 192, TM_O1 = 256, TM_U = 320, TM_U2 = 384, TM_G = 416, TM_UM = 480, TM_COLS = 512;
 
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ void bar_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory"); }
@@ -617,7 +622,7 @@ __device__ __forceinline__ void rk_issue(uint8_t *sm, RkCtl *ctl, int32_t beg, i
             for (int term = 0; term < terms; term++)
 #pragma unroll
                 for (int kk = 0; kk < 8; kk++)
-                    rk_mma(tm + d, tm + (term < 2 ? TM_S + 64 * (kk >> 2) + 32 * term : TM_S2 + 32 * (kk >> 2)) + 8 * (kk & 3),
+                    rk_mma(tm + d, tm + (term < 2 ? TM_S + 64 * (kk >> 2) + 32 * term : kk >> 2 ? TM_U2 : TM_S2) + 8 * (kk & 3),
                            b + (((kk >> 2) * RK_KSUB + (kk & 3) * 32) >> 4), rk_idesc(64, true, false), term + kk > 0);
         };
         if (one) {
@@ -669,7 +674,7 @@ __device__ __forceinline__ void rk_issue(uint8_t *sm, RkCtl *ctl, int32_t beg, i
             for (int term = 0; term < 3; term++)
 #pragma unroll
                 for (int ks = 0; ks < 4; ks++)
-                    rk_mma(tm + TM_U, tm + (term == 1 ? TM_UM : TM_S2 + 32) + 8 * ks, (term == 2 ? pm : ph) + (32 * ks >> 4), rk_idesc(64, true, false), term + ks > 0);
+                    rk_mma(tm + TM_U, tm + (term == 1 ? TM_UM : TM_UL) + 8 * ks, (term == 2 ? pm : ph) + (32 * ks >> 4), rk_idesc(64, true, false), term + ks > 0);
             rk_commit(&ctl->bar[3]);
         }
         __syncwarp();
@@ -796,7 +801,7 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
             }
             tm_st8(tl + TM_S + 64 * half + 8 * b, w0);
             tm_st8(tl + TM_S + 64 * half + 32 + 8 * b, w1);
-            if (DELTA) tm_st8(tl + TM_S2 + 32 * half + 8 * b, w2);
+            if (DELTA) tm_st8(tl + (half ? TM_U2 : TM_S2) + 8 * b, w2);
         }
         hand_over(BAR_HAND);
         if (DELTA) read_last();
@@ -891,7 +896,7 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
                 w0[i] = take_bf16(x, y);
                 w1[i] = take_bf16(x, y);
             }
-            tm_st8(tl + TM_S2 + 32 + 16 * half + 8 * b, w0);
+            tm_st8(tl + TM_UL + 16 * half + 8 * b, w0);
             tm_st8(tl + TM_UM + 16 * half + 8 * b, w1);
         }
         hand_over(BAR_HAND_U);
