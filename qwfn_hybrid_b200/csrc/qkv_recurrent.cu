@@ -252,6 +252,8 @@ __global__ void __launch_bounds__(RC_THREADS, 2) k_rec_conv(const __grid_constan
         int32_t beg, end;   // rows of the sequence
         const int i = rec_find(cu, p.n_seq, p.n_rows, r, beg, end);
         if (i < 0 || (r > beg && r < beg + RC_HIST)) {   // of no sequence (of this launch), or of the walk that holds its first row
+            // Row r's copy must have arrived: the next one goes to the same slot, and of two on their way either may be last.
+            asm volatile("cp.async.wait_group %0;" ::"n"(RC_AHEAD - 1) : "memory");
             fetch(r + RC_AHEAD);
             r++;
             continue;
