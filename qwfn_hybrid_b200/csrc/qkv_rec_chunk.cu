@@ -612,7 +612,10 @@ __device__ __forceinline__ void rk_issue(uint8_t *sm, RkCtl *ctl, int32_t beg, i
     for (int c = 0, st = 0; c < n_chunks; c++, st = st == RK_STAGES - 1 ? 0 : st + 1) {
         const uint32_t su = smu + st * RK_STAGE;
         bar_sync(BAR_FULL + st, RK_FULL_N);
-        if (reinterpret_cast<const float *>(sm + st * RK_STAGE + RK_COEF)[CF_N * RK_C + 1] != 0.0f) continue;
+        if (reinterpret_cast<const float *>(sm + st * RK_STAGE + RK_COEF)[CF_N * RK_C + 1] != 0.0f) {
+            bar_arrive(BAR_CHAIN, RK_HAND_N);   // the flag has been read: the chain may release the stage
+            continue;
+        }
         const uint64_t kq = rk_desc(su + RK_KQ, 16), kt = rk_desc(su + RK_KQ, RK_KSUB);
         const uint64_t th = rk_desc(su + RK_TH, 16), tl = rk_desc(su + RK_TL, 16), ph = rk_desc(su + RK_PH, 16), pm = rk_desc(su + RK_PM, 16);
         bar_sync(BAR_HAND, RK_HAND_N);
@@ -780,7 +783,7 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
             read_last();
             finish_out();
             store_state();
-            bar_sync(BAR_CHAIN, RK_CHAIN);
+            bar_sync(BAR_CHAIN, RK_HAND_N);   // and the issuer has read the flag, which the stage's next chunk clears
             load_v(t0 + RK_C);
             if (half == 0) rk_serial<DELTA>(p, S0, h, row, t0, min(end, t0 + RK_C));
             bar_sync(BAR_CHAIN, RK_CHAIN);

@@ -56,3 +56,23 @@ def test_full_grid_is_the_same_every_time(cuda, qkvlib, delta):
     beta = beta if delta else None
     S0, S1, out = run(qkvlib, LENGTHS, q, k, v, g, beta, **FULL, times=8)
     rec_bounds.check(S0, S1, LENGTHS, q, k, v, g, beta, out, SCALE)
+
+
+@pytest.mark.parametrize("delta", [True, False])
+def test_chunks_worked_token_by_token_among_others(cuda, qkvlib, delta):
+    """A growing state (g > 0) sends a chunk down the path token by token: none, every, every second, third and fourth chunk
+    of a head, three in a row, the first and the last."""
+    lengths = [700, 577, 640, 833]
+    q, k, v, g, beta = inputs(94, sum(lengths), FULL["H"], FULL["Hk"], torch.bfloat16, decay=0.02)
+    at = 0
+    for i, n in enumerate(lengths):
+        chunks = (n + 63) // 64
+        for h in range(FULL["H"]):
+            kind = (h + i) % 8
+            for c in range(chunks):
+                if (kind in (1, 2, 3, 4) and c % kind == (h // 8) % kind) or (kind == 5 and c in (3, 4, 5)) or (kind == 6 and c in (0, chunks - 1)):
+                    g[at + min(c * 64 + (5 * h + 11 * c) % 64, n - 1), h] = 0.01
+        at += n
+    beta = beta if delta else None
+    S0, S1, out = run(qkvlib, lengths, q, k, v, g, beta, **FULL, times=4)
+    rec_bounds.check(S0, S1, lengths, q, k, v, g, beta, out, SCALE)
