@@ -415,6 +415,7 @@ __device__ __forceinline__ void rk_produce(const RecParams &p, uint8_t *sm, RkCt
         bar_sync(BAR_PROD + grp, RK_GT);
         if (tid == RK_GT - 1) {   // scores: [k; q] k^T, once the other group has read its own
             if (c > 0) rk_wait_one(&ctl->read, (c - 1) & 1, ctl, p.status);
+            tc_fence_after();   // its loads of tensor memory come before the products that replace what they read
             const uint64_t kq = rk_desc(su + RK_KQ, 16);
 #pragma unroll
             for (int kk = 0; kk < 8; kk++) {

@@ -76,3 +76,22 @@ def test_chunks_worked_token_by_token_among_others(cuda, qkvlib, delta):
     beta = beta if delta else None
     S0, S1, out = run(qkvlib, lengths, q, k, v, g, beta, **FULL, times=4)
     rec_bounds.check(S0, S1, lengths, q, k, v, g, beta, out, SCALE)
+
+
+@pytest.mark.parametrize("delta", [True, False])
+def test_scores_of_another_size_in_each_chunk(cuda, qkvlib, delta):
+    """Two producer groups take turns with the columns of the scores: q (and without the delta rule k) a hundred times as
+    large in every second chunk, so that a score of another chunk shows."""
+    lengths = [1344, 1217, 1281, 1400]
+    q, k, v, g, beta = inputs(95, sum(lengths), FULL["H"], FULL["Hk"], torch.bfloat16, decay=0.02)
+    at = 0
+    for i, n in enumerate(lengths):
+        odd = (torch.arange(n, device="cuda") // 64 + i) % 2 == 1
+        size = torch.where(odd, 128.0, 1.0).bfloat16()[:, None]
+        q[at:at + n] *= size
+        if not delta:
+            k[at:at + n] *= size
+        at += n
+    beta = beta if delta else None
+    S0, S1, out = run(qkvlib, lengths, q, k, v, g, beta, **FULL, times=4)
+    rec_bounds.check(S0, S1, lengths, q, k, v, g, beta, out, SCALE)
