@@ -28,7 +28,9 @@
 //
 // A zero of T or P times a NaN is a NaN, so a chunk with a non-finite input would spread it to earlier
 // tokens; such chunks (and those with g > 0, a growing state, which could leave the range of what is scaled) are
-// flagged by the producers and run token by token from global memory.
+// flagged by the producers and run token by token from global memory.  Finite inputs can leave F32's range inside a chunk too
+// (long keys, repeated): a value row whose u is finite at its first token and not at a later one has the chunk thrown away and
+// run so.  (A row that starts with a state that is not finite has no output to save.)
 //
 // What bounds it: neither bytes nor the tensor cores (56 products of 32 or 64 cycles a chunk) but the chain's latency -- four
 // round trips from registers through tensor memory and a product a chunk -- and, beside it on the same schedulers, the
@@ -73,7 +75,8 @@ struct RkCtl {
     uint32_t tmem;
     int32_t  abort;
     int32_t  seq;
-    float    scale[128];      // inverse scale of R's first 32 tokens, per value row
+    int32_t  redo;            // the chunk's U left F32's range behind a value row's first token
+    float    scale[128];      // inverse scale of R's first 32 tokens, per value row (NaN: not finite from the first token on)
 };
 constexpr int RK_CTL = RK_VS + RK_C * REC_HD * 2;
 constexpr int RK_SMEM = RK_CTL + (int)sizeof(RkCtl);
@@ -812,6 +815,8 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
         else finish_out();
         // R = beta (v - e^G X), or u = v: tokens 32 half ..
         float X[32];
+        bool row_ok = true;
+        __nv_bfloat162 gone = __float2bfloat162_rn(0.0f);   // NaN once a value of w U is not finite
         const uint16_t *vs = reinterpret_cast<const uint16_t *>(sm + RK_VS) + 32 * half * 128 + row;
         if (DELTA) {
             rk_wait(&ctl->bar[0], ph, ctl, p.status);
@@ -829,6 +834,7 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
                 mx = fmaxf(fmaxf(mx, fmaxf(fabsf(X[i]), fabsf(X[i + 1]))), fmaxf(fabsf(X[i + 2]), fabsf(X[i + 3])));
             }
             const float s = pow2_scale(mx, inv);
+            if (half == 0 && !(fabsf(X[0]) <= 3.0e38f)) inv = __int_as_float(0x7fffffff);
 #pragma unroll
             for (int b = 0; b < 2; b++) {
                 uint32_t hi[8], lo[8];
@@ -845,12 +851,14 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
             tm_wait_ld(X);
             if (half) {
                 const float first = ctl->scale[row];
+                row_ok = first == first;
                 float Y[32];
                 tm_ld32(tl + TM_U2, Y);
                 tm_wait_ld(Y);
 #pragma unroll
                 for (int i = 0; i < 32; i++) X[i] = fmaf(first, X[i], inv * Y[i]);
             } else {
+                row_ok = inv == inv;
 #pragma unroll
                 for (int i = 0; i < 32; i++) X[i] *= inv;
             }
@@ -883,12 +891,16 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
                 w1[i + 1] = take_bf16(x, y);
                 w2[i + 1] = take_bf16(x, y);
             }
+            if (DELTA)
+#pragma unroll
+                for (int i = 0; i < 8; i++) gone = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&w0[i]), __float2bfloat162_rn(0.0f), gone);
             tm_st8(tl + TM_X + 32 * half + 8 * b, w0);
             tm_st8(tl + TM_X + 32 * half + 16 + 8 * b, w1);
             tm_st8(tl + TM_S2 + 16 * half + 8 * b, w2);
         }
         // (With the delta rule two waits for products lie between a chunk's hand-overs on one barrier.  Without it nothing does: a
         // fast warp's second arrival must not stand for a slow one's first.)
+        if (DELTA && row_ok && (*reinterpret_cast<const uint32_t *>(&gone) & 0x7fff7fffu)) *(volatile int32_t *)&ctl->redo = 1;
         hand_over(DELTA ? BAR_HAND : BAR_CHAIN);
         // U in two terms for the output
 #pragma unroll
@@ -907,6 +919,18 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
         if (DELTA) finish_out();
         const float eg = cf[CF_N * RK_C];
         rk_wait(&ctl->bar[2], ph, ctl, p.status);
+        if (DELTA && *(volatile int32_t *)&ctl->redo) {   // (written before the hand-over that bar[2] stands behind: all see the same)
+            rk_wait(&ctl->bar[3], ph, ctl, p.status);   // nothing reads the stage or U's terms any more
+            store_state();
+            bar_sync(BAR_CHAIN, RK_CHAIN);
+            if (tid == 0) ctl->redo = 0;
+            if (half == 0) rk_serial<DELTA>(p, S0, h, row, t0, min(end, t0 + RK_C));
+            bar_sync(BAR_CHAIN, RK_CHAIN);
+            load_state();
+            release(c);
+            ph ^= 1;
+            continue;
+        }
         if (!DELTA) load_v(t0 + RK_C);   // (every thread has read its part)
 #pragma unroll
         for (int b = 0; b < 2; b++) {
@@ -966,6 +990,7 @@ __global__ void __launch_bounds__(RK_THREADS, 1) k_rec_chunk(const __grid_consta
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     } else if (threadIdx.x == 0) {
         ctl->abort = 0;
+        ctl->redo = 0;
         for (int i = 0; i < RK_BARS + RK_GROUPS; i++)
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(i < RK_BARS ? &ctl->bar[i] : &ctl->scored[i - RK_BARS])) : "memory");
         asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(&ctl->read)), "r"(RK_GT) : "memory");

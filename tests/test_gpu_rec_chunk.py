@@ -95,3 +95,56 @@ def test_scores_of_another_size_in_each_chunk(cuda, qkvlib, delta):
     beta = beta if delta else None
     S0, S1, out = run(qkvlib, lengths, q, k, v, g, beta, **FULL, times=4)
     rec_bounds.check(S0, S1, lengths, q, k, v, g, beta, out, SCALE)
+
+
+@pytest.mark.parametrize("at", [0, 3, 31, 33, 62, 64, 100, 190])
+def test_finite_inputs_that_leave_the_range_late_in_a_chunk(cuda, qkvlib, at):
+    """One key of length 10^6, repeated from row `at` on: the delta rule multiplies the state by 10^12 a token and F32 is left a
+    few tokens on.  Rows before that keep their outputs, other heads are not touched, rows behind it are not finite."""
+    lengths, H = [64, 200, 130], 3
+    rows = sum(lengths)
+    q, k, v, g, beta = inputs(96, rows, H, H, torch.bfloat16, decay=0.02)
+    first = 64 + at                                     # in the second sequence, head 1
+    k[first:264, HD:2 * HD] = k[first, HD:2 * HD] * 2 ** 20
+    beta[first:264, 1] = 1.0
+    S0, S1, out = run(qkvlib, lengths, q, k, v, g, beta, H, H, times=2)
+    head = lambda x, h: x[:, h * HD:(h + 1) * HD]       # noqa: E731
+    for h in (0, 2):
+        rec_bounds.check(S0[:, h:h + 1], S1[:, h:h + 1], lengths, head(q, h), head(k, h), head(v, h), g[:, h:h + 1], beta[:, h:h + 1], out[:, h:h + 1], SCALE)
+    for i, r in ((0, slice(0, 64)), (2, slice(264, 394))):
+        rec_bounds.check(S0[i:i + 1, 1:2], S1[i:i + 1, 1:2], [lengths[i]], head(q[r], 1), head(k[r], 1), head(v[r], 1), g[r, 1:2], beta[r, 1:2], out[r, 1:2], SCALE)
+    # token by token in 64 bits: the largest value of the state and of what makes it, per value row
+    S, high = S0[1, 1].double(), torch.zeros(HD, dtype=torch.float64, device="cuda")
+    for t in range(64, 264):
+        kt, before = head(k, 1)[t].double(), high.clone()
+        S = S * torch.exp(g[t, 1].double())
+        u = beta[t, 1].double() * (head(v, 1)[t].double() - S @ kt)
+        S = S + u[:, None] * kt
+        high = torch.maximum(before, torch.maximum(S.abs().amax(1), u.abs() * kt.abs().amax()))
+        finite = torch.isfinite(out[t, 1].float())
+        assert bool(finite[high < 1e36].all()), f"row {t - 64}"
+        assert not bool(finite[before > 1e42].any()), f"row {t - 64}"
+        if bool((high < 1e36).all()):
+            last = t + 1
+    n = last - 64
+    assert at <= n < at + 12
+    if n:
+        o, _, bound, _ = rec_bounds.sequence(S0[1, 1:2], *(head(x, 1)[64:last] for x in (q, k, v)), g[64:last, 1:2], beta[64:last, 1:2], SCALE)
+        assert bool(((out[64:last, 1:2].double() - o).abs() <= bound).all())
+    assert not torch.isfinite(S1[1, 1]).any()
+
+
+def test_a_state_that_is_not_finite_stays_in_its_value_rows(cuda, qkvlib):
+    lengths, H = [300, 200], 2
+    q, k, v, g, beta = inputs(97, sum(lengths), H, 1, torch.bfloat16, decay=0.02)
+    S0 = torch.randn(2, H, HD, HD, generator=torch.Generator().manual_seed(98)).cuda() * 0.3
+    bad = S0.clone()
+    bad[0, 1, 5, 7], bad[0, 1, 77, 100], bad[1, 0, 3, 3] = float("nan"), float("inf"), -float("inf")
+    for d in (beta, None):
+        _, S1, out = run(qkvlib, lengths, q, k, v, g, d, H, 1, S0=bad, times=2)
+        rest = torch.ones(2, H, HD, dtype=torch.bool, device="cuda")
+        rest[0, 1, 5] = rest[0, 1, 77] = rest[1, 0, 3] = False
+        mask = torch.repeat_interleave(rest, torch.tensor(lengths, device="cuda"), 0)
+        assert torch.isfinite(S1[rest]).all() and torch.isfinite(out[mask].float()).all() and not torch.isfinite(out[~mask].float()).any()
+        _, S2, clean = run(qkvlib, lengths, q, k, v, g, d, H, 1, S0=S0)
+        assert torch.equal(S1[rest], S2[rest]) and torch.equal(out[mask], clean[mask])
