@@ -1407,6 +1407,7 @@ extern "C" qkv_status qkv_batch_map(qkv_engine *eng, const int32_t *slots, const
     if ((r = check_slots(eng, slots, n_seq, "batch_map")) != QKV_OK) return r;
     int64_t total = 0;
     size_t need = 0;
+    std::vector<int32_t> shared;
     for (int32_t i = 0; i < n_seq; i++) {
         const qkv_engine::Slot &sl = eng->slots[slots[i]];
         if (n_new[i] < 0 || pos0[i] < 0 || pos0[i] > sl.n_past)
@@ -1414,8 +1415,16 @@ extern "C" qkv_status qkv_batch_map(qkv_engine *eng, const int32_t *slots, const
         if ((int64_t)pos0[i] + n_new[i] > eng->cfg.n_ctx)
             return fail(eng, QKV_ERR_STATE, "context exhausted: %d + %d > n_ctx %d", pos0[i], n_new[i], eng->cfg.n_ctx);
         total += n_new[i];
-        for (int32_t pi = pos0[i] / PAGE_TOK; n_new[i] > 0 && pi <= (pos0[i] + n_new[i] - 1) / PAGE_TOK; pi++)
-            if (pi >= (int32_t)sl.pages.size() || eng->refcnt[sl.pages[pi]] > 1) need++;
+        for (int32_t pi = pos0[i] / PAGE_TOK; n_new[i] > 0 && pi <= (pos0[i] + n_new[i] - 1) / PAGE_TOK; pi++) {
+            if (pi >= (int32_t)sl.pages.size()) need++;
+            else if (eng->refcnt[sl.pages[pi]] > 1) shared.push_back(sl.pages[pi]);
+        }
+    }
+    // A shared page is copied once per slot that writes it, but the last of all its holders keeps it.
+    std::sort(shared.begin(), shared.end());
+    for (size_t i = 0, j; i < shared.size(); i = j) {
+        for (j = i; j < shared.size() && shared[j] == shared[i]; j++) {}
+        need += std::min(j - i, (size_t)eng->refcnt[shared[i]] - 1);
     }
     if (total > n_rows) return fail(eng, QKV_ERR_INVALID, "batch_map: %lld new rows, outputs hold %d", (long long)total, n_rows);
     if (need > eng->free_pages.size())
