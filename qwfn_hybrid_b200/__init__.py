@@ -150,19 +150,21 @@ def lib() -> ctypes.CDLL:
 
 
 def _i32_array(values) -> ctypes.Array:
-    n = len(values)
+    vals = values if type(values) in (list, tuple) else list(values)   # (iterators; array.array takes bytes for its items' memory)
+    n = len(vals)
     try:   # a few times cheaper than a ctypes constructor per value
-        return (ctypes.c_int32 * n).from_buffer(array.array("i", values)) if n else (ctypes.c_int32 * 1)()
+        return (ctypes.c_int32 * n).from_buffer(array.array("i", vals)) if n else (ctypes.c_int32 * 1)()
     except (TypeError, OverflowError):
-        return (ctypes.c_int32 * max(1, n))(*[int(v) for v in values])
+        return (ctypes.c_int32 * max(1, n))(*[int(v) for v in vals])
 
 
 def _i32s(values) -> array.array:
     """int32 values whose buffer_info()[0] is passed as a pointer while the array lives (cheaper than a ctypes array)."""
+    vals = values if type(values) in (list, tuple) else list(values)
     try:
-        return array.array("i", values)
+        return array.array("i", vals)
     except TypeError:
-        return array.array("i", [int(v) for v in values])
+        return array.array("i", [int(v) for v in vals])
 
 
 def _ptr(x) -> int | None:
