@@ -40,9 +40,9 @@ def spectral(Phi):
     return torch.exp(log / 2)
 
 
-def sequence(S, q, k, v, g, beta, scale):
+def sequence(S, q, k, v, g, beta, scale, piece=1 << 30):
     """One sequence from state S [heads, value, key].  Returns the 64-bit outputs [n, heads, 128] and last state, the
-    outputs' bound (same shape) and the state's, a norm per head."""
+    outputs' bound (same shape) and the state's, a norm per head.  piece: rows of a call, where chunks begin anew."""
     S, g = S.double(), g.double()
     q, k, v = _rows(q), _rows(k), _rows(v)
     n, heads = v.shape[0], v.shape[1]
@@ -51,8 +51,8 @@ def sequence(S, q, k, v, g, beta, scale):
     e = torch.exp(g)
     out, bound = torch.empty_like(v), torch.empty_like(v)
     E = torch.zeros(heads, dtype=torch.float64, device=v.device)
-    for t0 in range(0, n, C):
-        r = slice(t0, min(t0 + C, n))
+    for t0 in (t for a in range(0, n, piece) for t in range(a, min(a + piece, n), C)):
+        r = slice(t0, min(t0 + C, t0 - t0 % piece + piece, n))
         m = r.stop - t0
         S0, us = S, []
         Phi = torch.eye(HD, dtype=torch.float64, device=v.device).expand(heads, HD, HD)

@@ -148,3 +148,70 @@ def test_a_state_that_is_not_finite_stays_in_its_value_rows(cuda, qkvlib):
         assert torch.isfinite(S1[rest]).all() and torch.isfinite(out[mask].float()).all() and not torch.isfinite(out[~mask].float()).any()
         _, S2, clean = run(qkvlib, lengths, q, k, v, g, d, H, 1, S0=S0)
         assert torch.equal(S1[rest], S2[rest]) and torch.equal(out[mask], clean[mask])
+
+
+@pytest.mark.parametrize("lengths,n_keys,low", [([64], 1, 1.0), ([200, 64, 7], 1, 1.0), ([1000], 4, 1.0), ([333, 128], 2, 0.5), ([150], 1, 2.0), ([257], 3, 0.0)])
+def test_repeated_keys(cuda, qkvlib, lengths, n_keys, low):
+    """Few keys over and over (padding, repeated tokens), write strengths of `low` to low + 1 (2: two always, where each write
+    mirrors the state): the inverse T is far from the identity, no token lengthens an error."""
+    H, rows = 3, sum(lengths)
+    q, k, v, g, beta = inputs(101, rows, H, H, torch.bfloat16, decay=0.002)
+    pick = torch.randint(n_keys, (rows,), generator=torch.Generator().manual_seed(102)).cuda()
+    k.copy_(k[pick])
+    beta = torch.full_like(beta, 2.0) if low == 2.0 else beta + low
+    S0, S1, out = run(qkvlib, lengths, q, k, v, g, beta, H, H, times=2)
+    rec_bounds.check(S0, S1, lengths, q, k, v, g, beta, out, SCALE)
+
+
+@pytest.mark.parametrize("delta", [True, False])
+@pytest.mark.parametrize("size,at,n", [(1.75, 0, 700), (1.75, 100, 200), (1.25, 0, 2400), (3.0, 30, 40)])
+def test_long_keys(cuda, qkvlib, size, at, n, delta):
+    """Keys longer than one: with the delta rule a token may lengthen what it meets."""
+    rows, H = 2400 if n > 700 else 700, 2
+    q, k, v, g, beta = inputs(103, rows, H, 1, torch.bfloat16, decay=1e-2)
+    k[at:at + n] *= size
+    beta = beta if delta else None
+    S0, S1, out = run(qkvlib, [rows], q, k, v, g, beta, H, 1)
+    rec_bounds.check(S0, S1, [rows], q, k, v, g, beta, out, SCALE)
+
+
+@pytest.mark.parametrize("piece", [2400, 333])
+@pytest.mark.parametrize("what", ["nan in v", "inf in k", "nan in q", "nan in beta"])
+@pytest.mark.parametrize("at", [0, 1023, 2000])
+def test_values_that_are_not_finite_against_the_definition(cuda, qkvlib, what, at, piece):
+    """The rows and value rows that the 64-bit recurrence leaves finite are finite and within bounds, and no others; in calls whose
+    chunks begin at other rows too."""
+    rows, H = 2400, 2
+    q, k, v, g, beta = inputs(104, rows, H, 2, torch.bfloat16, decay=1e-2)
+    where, value = what.split(" in ")[1], float(what.split(" ")[0])
+    if where == "beta":
+        beta[at, 1] = value
+    else:
+        dict(q=q, k=k, v=v)[where][at, HD + 5] = value
+    eng = engine(qkvlib, H, 1, 2)
+    S0 = torch.randn(1, H, HD, HD, generator=torch.Generator().manual_seed(105)).cuda() * 0.3
+    eng.rec_state(0).copy_(S0)
+    out = torch.full((rows, H, HD), 7.0, dtype=torch.bfloat16, device="cuda")
+    for a in range(0, rows, piece):
+        r = slice(a, min(a + piece, rows))
+        eng.rec_chunk(0, [0], offsets([r.stop - r.start]), q[r], k[r], v[r], g[r], beta[r], SCALE, out[r])
+    torch.cuda.synchronize()
+    S1 = eng.rec_state(0)
+    head = lambda x, h: x[:, h * HD:(h + 1) * HD]       # noqa: E731
+    # the other head as if nothing were there, and this one up to the row
+    o, S, bound, E = rec_bounds.sequence(S0[0, :1], *(head(x, 0) for x in (q, k, v)), g[:, :1], beta[:, :1], SCALE, piece)
+    assert bool(((out[:, :1].double() - o).abs() <= bound).all())
+    assert bool(((S1[0, :1].double() - S).flatten(1).norm(dim=1) <= E).all())
+    if at:
+        o, _, bound, _ = rec_bounds.sequence(S0[0, 1:], *(head(x, 1)[:at] for x in (q, k, v)), g[:at, 1:], beta[:at, 1:], SCALE, piece)
+        assert bool(((out[:at, 1:].double() - o).abs() <= bound).all())
+    # from the row on: finite where the definition is
+    S, finite = S0[0, 1].double(), torch.empty(rows, HD, dtype=torch.bool, device="cuda")
+    for t in range(rows):
+        kt = head(k, 1)[t].double()
+        S = S * torch.exp(g[t, 1].double())
+        u = beta[t, 1].double() * (head(v, 1)[t].double() - S @ kt)
+        S = S + u[:, None] * kt
+        finite[t] = torch.isfinite(S @ head(q, 1)[t].double())
+    assert torch.equal(torch.isfinite(out[:, 1].float()), finite)
+    assert torch.equal(torch.isfinite(S1[0, 1]), torch.isfinite(S))
