@@ -245,6 +245,10 @@ __global__ void __launch_bounds__(RC_THREADS, 2) k_rec_conv(const __grid_constan
         w[e][0] = u.x; w[e][1] = u.y; w[e][2] = u.z; w[e][3] = u.w;
     }
     __syncthreads();
+    if (r_hi <= cu[0] || r_lo >= cu[p.n_seq]) {   // rows of other launches' sequences alone
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        return;
+    }
     const bool norm = c0 < p.n_norm;
     const float max_inv = 1.0f / p.eps;
     const unsigned lanes = rec_head_lanes<T>();
