@@ -320,8 +320,8 @@ typedef enum qkv_dtype { QKV_F32 = 0, QKV_BF16 = 1 } qkv_dtype;
  * the rows before a sequence's first being its history (state kind 1: [channel][3], oldest first),
  * which then holds its last three rows; of the first n_norm channels (a multiple of 128: the heads of q
  * and k) every 128 are divided by max(their 2-norm, eps).  cu: device int32 [n_seq+1] row offsets
- * (qkv_batch_map); rows outside the sequences are neither read nor written, a sequence without rows
- * keeps its state.  x: device rows of conv_channels values of `dtype`, x_stride elements apart; y:
+ * (qkv_batch_map); rows outside the sequences are not written, and their values enter nothing (they may be read: x
+ * holds n_rows rows); a sequence without rows keeps its state.  x: device rows of conv_channels values of `dtype`, x_stride elements apart; y:
  * device [n_rows][conv_channels] of the same type, not overlapping x; w: device F32
  * [conv_channels][4].  Pointers 16-byte aligned, x_stride a multiple of 16 bytes. */
 qkv_status qkv_rec_conv(qkv_engine *eng, int32_t rec_layer, const int32_t *slots, const int32_t *cu, int32_t n_seq,
@@ -329,7 +329,7 @@ qkv_status qkv_rec_conv(qkv_engine *eng, int32_t rec_layer, const int32_t *slots
                         int32_t n_norm, float eps, void *y, int32_t save, void *stream);
 
 /* Rows of linear attention: value head h of rec_n_head reads head h / (rec_n_head / n_head_k) of q and
- * k.  Row r's q and k are n_head_k heads of 128 at q + r * q_stride (elements), its v rec_n_head heads
+ * k (neighbouring value heads share one; there is no other order).  Row r's q and k are n_head_k heads of 128 at q + r * q_stride (elements), its v rec_n_head heads
  * of 128 at v + r * v_stride; slices of one fused row are allowed.  g: F32 [rows][rec_n_head], the log
  * of each head's decay (-inf allowed: the state is forgotten; +inf and NaN are not); beta: F32
  * [rows][rec_n_head] for the gated delta rule, NULL for decay alone.  All device; q, k, v 16-byte
@@ -351,7 +351,9 @@ qkv_status qkv_rec_step(qkv_engine *eng, int32_t rec_layer, const int32_t *slots
                         const qkv_rec_rows *rows, int32_t T, float scale, float *out, int32_t save, void *stream);
 /* Chunked form for prompts: the same recurrence over ragged rows, cu as in qkv_rec_conv; q, k, v: bf16
  * rows; out: bf16 [n_rows][rec_n_head][128].  State, sums and decays are F32; out is rounded once
- * at the end.  A row offset outside 0 .. n_rows, or a falling one, skips that sequence and sets the
+ * at the end.  The products' operands are split into terms: u = beta * (v - S k) of a value row keeps 22 bits, and none below
+ * 2^-38 of the largest u of its 32 tokens.  A value that is not finite, or that leaves F32's range on the way, changes no row
+ * before its own and no head or value row that does not depend on it.  A row offset outside 0 .. n_rows, or a falling one, skips that sequence and sets the
  * bad-index bit of qkv_device_status. */
 qkv_status qkv_rec_chunk(qkv_engine *eng, int32_t rec_layer, const int32_t *slots, const int32_t *cu, int32_t n_seq,
                          const qkv_rec_rows *rows, int32_t n_rows, float scale, uint16_t *out, void *stream);

@@ -21,8 +21,9 @@
 //
 // Precision.  k and q are exact in bf16, so S, w U and U enter as sums of bf16 terms (three: 24 bits; two for what
 // only the rounded output sees, as P; truncated terms, which need no conversion: three of them are the value), and T
-// and R, which meet each other, as two f16 terms of rows scaled to [2^12, 2^13) (22 bits), three products: state and U
-// keep 32-bit accuracy (2 to 5e-7 of the state's norm against 64 bits).  Sums are F32; the state is scaled and added
+// and R, which meet each other, as two f16 terms of rows scaled to [2^12, 2^13) (22 bits; of T's row of a token, of R's
+// value row over 32 tokens: what is more than 2^16 below the row's largest loses bits, and below 2^-38 of it is lost),
+// three products: state and U keep 32-bit accuracy (2 to 5e-7 of the state's norm against 64 bits).  Sums are F32; the state is scaled and added
 // outside the tensor cores (their sums are truncated).  G is summed as pairs of floats: e^(G_i - G_j) needs the
 // difference, not the rounded sums.  The output is rounded to bf16 once.
 //
@@ -32,14 +33,15 @@
 // (long keys, repeated): a value row whose u is finite at its first token and not at a later one has the chunk thrown away and
 // run so.  (A row that starts with a state that is not finite has no output to save.)
 //
-// What bounds it: neither bytes nor the tensor cores (56 products of 32 or 64 cycles a chunk) but the chain's latency -- four
+// What bounds it: neither bytes nor the tensor cores (84 products of 32 or 64 cycles a chunk, 48 without the delta rule) but the chain's latency -- four
 // round trips from registers through tensor memory and a product a chunk -- and, beside it on the same schedulers, the
-// producers'.  A chunk takes 5.0 us (delta rule, 16384 tokens: 1280 us) or 3.5 us (decay alone).  From about 100
-// CTAs on it takes longer, 5.3 to 7.6 us: the three roles' loops are more instructions than an SM keeps, and the SMs of a group
-// fetch them from one cache (at 148 CTAs warps waited 3.5 cycles per instruction for instructions, at 32 CTAs 0.4).  So the
+// producers'.  A chunk takes 5.0 us (delta rule, 16384 tokens: 1278 us) or 3.3 us (decay alone).  From about 100
+// CTAs on it takes longer, 5.6 to 8.4 us at 148 CTAs with k and q of their own: the three roles' loops are more instructions than an SM keeps, and the SMs of a group
+// fetch them from one cache (at 148 CTAs warps waited 3.5 cycles per instruction for instructions, at 32 CTAs 0.4; with the
+// loops as they are, 1.6 and 0.3).  So the
 // code is kept short where time allows: one body for the rows of k and of q, loops over tiles of T and over the terms of a
-// product (24 prompts of 24001 rows, 32 heads: 656 -> 556 us); with all products in loops 148 equal CTAs take 6.4 us, but few of
-// them 5.4.  Not kept: a long sequence in three parts by clusters of three CTAs (the state is linear in the one it starts
+// product (24 prompts of 24001 rows, 32 heads: 656 -> 556 us); with all products in loops 148 equal CTAs took 16% less than so, but few of
+// them 3% more.  Not kept: a long sequence in three parts by clusters of three CTAs (the state is linear in the one it starts
 // from) took 1160 instead of 1310 us and, through its registers, made all other sizes 3 to 7% slower; a kernel of the same split on
 // mma.sync, 64 value rows per CTA, took 5.9 us per chunk and half a head.
 #include "qkv_internal.h"
