@@ -586,25 +586,67 @@ __device__ __forceinline__ void rk_produce(const RecParams &p, uint8_t *sm, RkCt
 }
 
 // ---- the chain
-// A flagged chunk, token by token, everything from global memory; a thread per value row.
+// A chunk token by token from global memory, by the chain's warps: 16 value rows each, 8 at a time in registers, 8 lanes a row as
+// in k_rec_step.
 template <bool DELTA>
-__device__ __noinline__ void rk_serial(const RecParams &p, float *S, int h, int dv, int32_t t0, int32_t t1) {
-    const int hk = h / (p.n_head / p.n_head_k);
-    for (int32_t r = t0; r < t1; r++) {
-        const __nv_bfloat16 *k = static_cast<const __nv_bfloat16 *>(p.k) + (int64_t)r * p.k_stride + hk * REC_HD;
-        const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q) + (int64_t)r * p.q_stride + hk * REC_HD;
-        const float eg = expf(p.g[(int64_t)r * p.n_head + h]);
-        float u = __bfloat162float(static_cast<const __nv_bfloat16 *>(p.v)[(int64_t)r * p.v_stride + h * REC_HD + dv]), d = 0.0f, o = 0.0f;
-        if (DELTA) {
-            for (int i = 0; i < REC_HD; i++) d = fmaf(S[i] * eg, __bfloat162float(k[i]), d);
-            u = p.beta[(int64_t)r * p.n_head + h] * (u - d);
+__device__ __noinline__ void rk_serial(const RecParams &p, float *state, int h, int32_t t0, int32_t t1) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, sub = lane & 7, hk = h / (p.n_head / p.n_head_k);
+#pragma unroll 1
+    for (int half = 0; half < 2; half++) {
+        const int row = wid * 16 + half * 8 + (lane >> 3);   // and row + 4
+        float *S0 = state + row * REC_HD + sub * 4;
+        float S[2][16];
+#pragma unroll
+        for (int a = 0; a < 2; a++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float4 x = *reinterpret_cast<const float4 *>(S0 + a * 4 * REC_HD + 32 * j);
+                S[a][4 * j] = x.x; S[a][4 * j + 1] = x.y; S[a][4 * j + 2] = x.z; S[a][4 * j + 3] = x.w;
+            }
+#pragma unroll 1
+        for (int32_t r = t0; r < t1; r++) {
+            float k[16], q[16];
+            auto load = [&](const void *x, int64_t stride, float (&o)[16]) {
+                const __nv_bfloat16 *at = static_cast<const __nv_bfloat16 *>(x) + r * stride + hk * REC_HD + sub * 4;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint2 w = *reinterpret_cast<const uint2 *>(at + 32 * j);
+                    o[4 * j] = __uint_as_float(w.x << 16); o[4 * j + 1] = __uint_as_float(w.x & 0xffff0000u);
+                    o[4 * j + 2] = __uint_as_float(w.y << 16); o[4 * j + 3] = __uint_as_float(w.y & 0xffff0000u);
+                }
+            };
+            load(p.k, p.k_stride, k);
+            load(p.q, p.q_stride, q);
+            const __nv_bfloat16 *v = static_cast<const __nv_bfloat16 *>(p.v) + r * p.v_stride + h * REC_HD + row;
+            float u[2] = {__bfloat162float(v[0]), __bfloat162float(v[4])}, o[2] = {};
+            const float eg = expf(p.g[(int64_t)r * p.n_head + h]), b = DELTA ? p.beta[(int64_t)r * p.n_head + h] : 1.0f;
+#pragma unroll
+            for (int a = 0; a < 2; a++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) S[a][i] *= eg;
+                if (DELTA) {
+                    float d = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) d = fmaf(S[a][i], k[i], d);
+#pragma unroll
+                    for (int m = 4; m; m >>= 1) d += __shfl_xor_sync(0xffffffffu, d, m);
+                    u[a] = b * (u[a] - d);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    S[a][i] = fmaf(u[a], k[i], S[a][i]);
+                    o[a] = fmaf(S[a][i], q[i], o[a]);
+                }
+#pragma unroll
+                for (int m = 4; m; m >>= 1) o[a] += __shfl_xor_sync(0xffffffffu, o[a], m);
+                if (sub == 0) static_cast<__nv_bfloat16 *>(p.out)[((int64_t)r * p.n_head + h) * REC_HD + row + 4 * a] = __float2bfloat16_rn(o[a] * p.scale);
+            }
         }
-        for (int i = 0; i < REC_HD; i++) {
-            const float s = fmaf(u, __bfloat162float(k[i]), S[i] * eg);
-            S[i] = s;
-            o = fmaf(s, __bfloat162float(q[i]), o);
-        }
-        static_cast<__nv_bfloat16 *>(p.out)[((int64_t)r * p.n_head + h) * REC_HD + dv] = __float2bfloat16_rn(o * p.scale);
+#pragma unroll
+        for (int a = 0; a < 2; a++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                *reinterpret_cast<float4 *>(S0 + a * 4 * REC_HD + 32 * j) = make_float4(S[a][4 * j], S[a][4 * j + 1], S[a][4 * j + 2], S[a][4 * j + 3]);
     }
 }
 
@@ -791,7 +833,7 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
             store_state();
             bar_sync(BAR_CHAIN, RK_HAND_N);   // and the issuer has read the flag, which the stage's next chunk clears
             load_v(t0 + RK_C);
-            if (half == 0) rk_serial<DELTA>(p, S0, h, row, t0, min(end, t0 + RK_C));
+            rk_serial<DELTA>(p, S0 - row * REC_HD, h, t0, min(end, t0 + RK_C));
             bar_sync(BAR_CHAIN, RK_CHAIN);
             load_state();
             release(c);
@@ -926,7 +968,7 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
             store_state();
             bar_sync(BAR_CHAIN, RK_CHAIN);
             if (tid == 0) ctl->redo = 0;
-            if (half == 0) rk_serial<DELTA>(p, S0, h, row, t0, min(end, t0 + RK_C));
+            rk_serial<DELTA>(p, S0 - row * REC_HD, h, t0, min(end, t0 + RK_C));
             bar_sync(BAR_CHAIN, RK_CHAIN);
             load_state();
             release(c);
