@@ -878,7 +878,7 @@ __device__ __forceinline__ void rk_chain(const RecParams &p, uint8_t *sm, RkCtl 
                 mx = fmaxf(fmaxf(mx, fmaxf(fabsf(X[i]), fabsf(X[i + 1]))), fmaxf(fabsf(X[i + 2]), fabsf(X[i + 3])));
             }
             const float s = pow2_scale(mx, inv);
-            if (half == 0 && !(fabsf(X[0]) <= 3.0e38f)) inv = __int_as_float(0x7fffffff);
+            if (half == 0 && !(fabsf(X[0]) < __int_as_float(0x7f800000))) inv = __int_as_float(0x7fffffff);
 #pragma unroll
             for (int b = 0; b < 2; b++) {
                 uint32_t hi[8], lo[8];

@@ -215,3 +215,17 @@ def test_values_that_are_not_finite_against_the_definition(cuda, qkvlib, what, a
         finite[t] = torch.isfinite(S @ head(q, 1)[t].double())
     assert torch.equal(torch.isfinite(out[:, 1].float()), finite)
     assert torch.equal(torch.isfinite(S1[0, 1]), torch.isfinite(S))
+
+
+def test_a_first_token_near_the_end_of_the_range(cuda, qkvlib):
+    """u of a chunk's first token between 3.0e38 and the largest F32 value is a number like any other."""
+    q, k, v, g, beta = inputs(106, 64, 1, 1, torch.bfloat16, decay=1e-3)
+    v[0, 5], v[0, 6] = 3.3e38, -3.2e38
+    v[1:] = 0
+    k.zero_()
+    k[0, 9] = 1.0
+    beta[0] = 1.0
+    S0 = torch.zeros(1, 1, HD, HD, device="cuda")
+    _, S1, out = run(qkvlib, [64], q, k, v, g, beta, 1, 1, S0=S0)
+    assert torch.isfinite(S1).all() and float(S1[0, 0, 5, 9]) > 2e38 and torch.isfinite(out.float()).all()
+    rec_bounds.check(S0, S1, [64], q, k, v, g, beta, out, SCALE)
